@@ -387,6 +387,81 @@ int rl_set_gemm_variant(int variant);
  * previous value. */
 int rl_set_attention_variant(int variant);
 
+/*
+ * The 8-bit paged cache of keys and values (no counterpart in the reference, whose text encoder keeps no cache), head
+ * dim 128. One layer of a pool is four arrays: codes pool_k / pool_v [pages][kv_heads][page][128] uint8 and exponents
+ * pool_ke / pool_ve [pages][kv_heads][page / 16] uint8; page = 16, 32, 64, 128 or 256 tokens. A block of 16 tokens of one
+ * head shares one exponent: value = (u - 128) * 2^(E - 133), u = code, and E = 255 reads as NaN.
+ *
+ * A batch of B <= 4096 sequences lies in device memory: table (B rows of table_ld int32: the pages of the sequence in
+ * order), kv_len[B] (tokens in the cache, the new ones included), q_start[B + 1] (the new tokens of sequence b are rows
+ * q_start[b] .. q_start[b + 1] - 1; row j of n sits at position kv_len - n + j). The kernels check what they read: a
+ * sequence whose numbers are impossible is left out, a page outside the pool is skipped (its keys count as absent), and
+ * both are reported through rl_device_status. Rows of no sequence are neither read nor written.
+ */
+
+/*
+ * Write the new tokens' keys and values. k, v: element (row, head, dim) at row * st + head * sh + dim * sd (elements),
+ * RL_BF16 or RL_F32. Per block, E becomes the larger of the older tokens' exponent and the new values' largest float32
+ * exponent field (older tokens: those before the new ones; a block without any starts from the new values alone); older
+ * codes are shifted by the difference, rounded half to even, and a new code is
+ * clip(rint_half_even(x * 2^(133 - E)), -128, 127) + 128. A NaN or an infinity makes E 255. Writing the same tokens
+ * again changes nothing. The pages that receive tokens must belong to one sequence of the batch only.
+ */
+int rl_kv_append(const void* k, int64_t k_st, int64_t k_sh, int64_t k_sd, const void* v, int64_t v_st, int64_t v_sh,
+                 int64_t v_sd, int dtype, int64_t T, uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke,
+                 uint8_t* pool_ve, int64_t pages, int kv_heads, int page, const int32_t* table, int64_t table_ld,
+                 const int32_t* kv_len, const int32_t* q_start, int B, rl_stream_t stream);
+
+/* Decode positions start[b] .. start[b] + count - 1 of each sequence into bf16 k_out, v_out (B, count, kv_heads, 128),
+ * exactly; zeros before 0 and at and after kv_len[b]. */
+int rl_kv_read(const uint8_t* pool_k, const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve,
+               int64_t pages, int kv_heads, int page, const int32_t* table, int64_t table_ld, const int32_t* kv_len,
+               const int32_t* start, int B, int64_t count, uint16_t* k_out, uint16_t* v_out, rl_stream_t stream);
+
+/* Copy page src[i] to page dst[i], i < n, in each of `layers` layers (layer strides pages * kv_heads * page * 128 and
+ * pages * kv_heads * page / 16). src, dst: host arrays, read before the call returns. The copies run at once, so a
+ * page that is written may be neither read nor written by another copy of the call (refused). */
+int rl_kv_copy_pages(uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke, uint8_t* pool_ve, int layers, int64_t pages,
+                     int kv_heads, int page, const int32_t* src, const int32_t* dst, int64_t n, rl_stream_t stream);
+
+/*
+ * Attention of the new tokens over the cache (grouped-query: query head h reads K/V head h / (heads / kv_heads)).
+ * q: bf16, element (row, head, dim) at row * q_st + head * q_sh + dim, strides multiples of 8, 16-byte aligned.
+ * Row j of n of a sequence sees the keys at positions <= kv_len - n + j, or, with row_limit (int32 [T]), those <=
+ * min(row_limit[row], kv_len - 1). A row that sees no key gives zeros. o: bf16 (T, ldo), head h at columns 128h ..,
+ * O / l rounded once (not to bfp16 blocks). Keys are weighted with P rounded to fp16; sums are fp32. Results do not
+ * depend on timing. workspace: rl_kv_attention_workspace bytes, 16-byte aligned, needs no initialisation and holds
+ * nothing between calls; calls that may run at the same time need workspaces of their own.
+ */
+size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads);
+int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, int heads, const uint8_t* pool_k,
+                    const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve, int64_t pages, int kv_heads,
+                    int page, const int32_t* table, int64_t table_ld, const int32_t* kv_len, const int32_t* q_start,
+                    int B, const int32_t* row_limit, float scale_log2, uint16_t* o, int64_t ldo, void* workspace,
+                    size_t workspace_bytes, rl_stream_t stream);
+
+/*
+ * 4-bit weights with group scales (no counterpart in the reference): B (K, N), value (u - 8) * s, u = 0 .. 15, one bf16
+ * scale per `group` (32, 64 or 128) consecutive k of a column; K % group == 0, any N.
+ * rl_w4_bytes: sizes of the native codes and scales. rl_w4_quantize: float B -> codes (K, N), one per byte, and scales
+ * (K / group, N): s = bf16(e / -8) with e the group's value of largest magnitude, u = clip(rint(w / s) + 8, 0, 15).
+ * rl_w4_pack: such codes and scales -> the native layout. swiglu_interleaved as in rl_pack_weights (N % 128 == 0).
+ */
+int rl_w4_bytes(int64_t K, int64_t N, int group, int swiglu_interleaved, size_t* code_bytes, size_t* scale_bytes);
+int rl_w4_quantize(const void* B, int dtype, int64_t K, int64_t N, int group, uint8_t* codes, uint16_t* scales,
+                   rl_stream_t stream);
+int rl_w4_pack(const uint8_t* codes, const uint16_t* scales, int64_t K, int64_t N, int group, int swiglu_interleaved,
+               uint8_t* w_out, uint8_t* s_out, rl_stream_t stream);
+
+/*
+ * C = x @ B (+ bias) for M <= 64 rows of bf16 x (M, K), 16-byte aligned, any bf16 values. Epilogues as rl_linear_bfp16
+ * (RL_EPI_SWIGLU: C (M, N / 2), rounded once to out_dtype and not to bfp16 blocks; a bias is optional there).
+ * Products are exact, sums fp32. Results do not depend on timing.
+ */
+int rl_linear_w4(const uint16_t* x, int64_t M, int64_t K, const uint8_t* w, const uint8_t* scales, int64_t N, int group,
+                 const uint16_t* bias, int epilogue, void* out, int out_dtype, rl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

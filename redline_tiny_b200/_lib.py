@@ -70,6 +70,17 @@ SIGNATURES = {
     "rl_ipc_close": (_I, [_P]),
     "rl_ipc_free": (_I, [_P]),
     "rl_tp_signal": (_I, [_P, _I, _I, _I, ctypes.c_ulonglong, _P]),
+    "rl_kv_append": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I, _I64, _P, _P, _P, _P, _I64, _I, _I, _P, _I64,
+                          _P, _P, _I, _P]),
+    "rl_kv_read": (_I, [_P, _P, _P, _P, _I64, _I, _I, _P, _I64, _P, _P, _I, _I64, _P, _P, _P]),
+    "rl_kv_copy_pages": (_I, [_P, _P, _P, _P, _I, _I64, _I, _I, _P, _P, _I64, _P]),
+    "rl_kv_attention_workspace": (ctypes.c_size_t, [_I64, _I, _I, _I]),
+    "rl_kv_attention": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _I, _P, _I64, _P, _P, _I, _P,
+                             ctypes.c_float, _P, _I64, _P, ctypes.c_size_t, _P]),
+    "rl_w4_bytes": (_I, [_I64, _I64, _I, _I, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
+    "rl_w4_quantize": (_I, [_P, _I, _I64, _I64, _I, _P, _P, _P]),
+    "rl_w4_pack": (_I, [_P, _P, _I64, _I64, _I, _I, _P, _P, _P]),
+    "rl_linear_w4": (_I, [_P, _I64, _I64, _P, _P, _I64, _I, _P, _I, _P, _I, _P]),
     "rl_ln_mod_tp": (_I, [_P, _P, _I, _P, _I, ctypes.c_ulonglong, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
 }
 

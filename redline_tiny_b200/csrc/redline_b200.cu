@@ -9,3 +9,6 @@
 #include "rl_adaln.cu"
 #include "rl_npu.cu"
 #include "rl_tp.cu"
+#include "rl_kv.cu"
+#include "rl_kv_attn.cu"
+#include "rl_w4.cu"

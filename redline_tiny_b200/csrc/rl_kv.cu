@@ -1,0 +1,404 @@
+// The 8-bit paged cache of keys and values: writing new tokens, reading positions back, copying pages.
+//
+// A page holds `page` tokens (16, 32, 64, 128 or 256) of every K/V head of one layer: codes [Hkv][page][128] and one
+// exponent byte per block of 16 tokens and head, [Hkv][page / 16]. A block is the bfp16 format with 16 x 128 values
+// instead of 8: value = (u - 128) * 2^(E - 133), u = m + 128 in offset binary (as the native weight tiles), E the
+// largest float32 exponent field in the block. The scale is a power of two because then every decoded value is exact
+// in bf16 (8 significant bits), and a block whose later tokens need a larger E is rewritten by a shift. E = 255 marks
+// a block that took in a NaN or an infinity; it reads as NaN.
+//
+// All three kernels are bound by bytes; the per-byte arithmetic is a few instructions.
+#include <cstdlib>
+
+#include "rl_common.cuh"
+#include "rl_host.h"
+
+namespace rl {
+namespace kv {
+
+constexpr int HD = 128;     // head dim
+constexpr int BT = 16;      // tokens per block (one exponent)
+constexpr int kMaxBatch = 4096;
+
+struct Pool {               // one layer
+  uint8_t *k, *v, *ke, *ve;
+  int64_t pages;
+  int hkv, page;
+};
+
+struct Batch {
+  const int32_t* table;     // (B, ld): page of each `page` tokens of each sequence
+  int64_t ld;
+  const int32_t* kv_len;    // (B): tokens in the cache, the new ones included
+  const int32_t* q_start;   // (B + 1): rows of the new tokens
+  int B;
+  int64_t T;                // rows
+};
+
+// One sequence of a batch, checked against the sizes that the host knows. An impossible one is reported and dropped.
+struct Seq {
+  int64_t s0, n, len;
+  bool ok;
+};
+__device__ __forceinline__ Seq load_seq(const Batch& bt, int b, int page) {
+  Seq s;
+  s.s0 = __ldg(bt.q_start + b);
+  s.n = __ldg(bt.q_start + b + 1) - s.s0;
+  s.len = __ldg(bt.kv_len + b);
+  s.ok = s.s0 >= 0 && s.n >= 0 && s.s0 + s.n <= bt.T && s.len >= s.n && s.len <= bt.ld * page;
+  return s;
+}
+
+// Index of the block (layer-wide) that holds token position `pos` of sequence b for head h, or -1 for a bad page.
+__device__ __forceinline__ int64_t block_index(const Pool& p, const Batch& bt, int b, int64_t pos, int h) {
+  const int64_t pg = __ldg(bt.table + b * bt.ld + pos / p.page);
+  if (pg < 0 || pg >= p.pages) return -1;
+  return (pg * p.hkv + h) * (p.page / BT) + (pos % p.page) / BT;
+}
+
+// m / 2^d for a code of an older token, rounded half to even (d >= 1), as an offset-binary byte.
+__device__ __forceinline__ uint32_t shift_code(uint32_t u, int d) {
+  const int m = static_cast<int>(u) - 128;
+  if (d >= 9) return 128u;
+  return static_cast<uint32_t>(((m + (1 << (d - 1)) - 1 + ((m >> d) & 1)) >> d) + 128);
+}
+
+struct Source {             // rows of new keys or values: element (t, h, d) at t * st + h * sh + d * sd
+  const void* x;
+  int64_t st, sh, sd;
+};
+
+// The 4 values of one token that a lane owns (dims 4 * lane ..), as float32 bits.
+template <typename X>
+__device__ __forceinline__ void load4(const Source& s, int64_t t, int h, int lane, bool vec, uint32_t (&b)[4]) {
+  const X* p = static_cast<const X*>(s.x) + t * s.st + h * s.sh + 4 * lane * s.sd;
+  if (sizeof(X) == 2) {
+    if (vec) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      b[0] = w.x << 16, b[1] = w.x & 0xFFFF0000u, b[2] = w.y << 16, b[3] = w.y & 0xFFFF0000u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + i * s.sd)) << 16;
+    }
+  } else {
+    if (vec) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint32_t*>(p + i * s.sd);
+    }
+  }
+}
+
+// One warp per (group of `rows` rows, head, K or V). A row leads when it is the first of its block among the new
+// tokens; the warp writes the blocks of its leading rows: the block's new values are read once into registers, their
+// largest exponent field is joined with the exponent of the older tokens of the block, and the codes are stored.
+template <typename X>
+__global__ void __launch_bounds__(128) append_kernel(const Source sk, const Source sv, const Pool p, const Batch bt,
+                                                     int rows, int64_t groups) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  if (w >= groups * p.hkv * 2) return;
+  const int is_v = static_cast<int>(w & 1);
+  const int h = static_cast<int>((w >> 1) % p.hkv);
+  const int64_t r0 = (w >> 1) / p.hkv * rows;
+  const Source src = is_v ? sv : sk;
+  uint8_t* codes = is_v ? p.v : p.k;
+  uint8_t* exps = is_v ? p.ve : p.ke;
+  const bool vec = src.sd == 1 && ((reinterpret_cast<uintptr_t>(src.x) | (src.st * sizeof(X)) | (src.sh * sizeof(X))) &
+                                   (4 * sizeof(X) - 1)) == 0;
+  // the sequence of row r0: the last b with q_start[b] <= r0
+  int lo = 0, hi = bt.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(bt.q_start + mid) <= r0) lo = mid; else hi = mid;
+  }
+  int b = lo;
+  Seq s = load_seq(bt, b, p.page);
+  for (int64_t r = r0; r < min(r0 + rows, bt.T);) {
+    while (b + 1 < bt.B && r >= s.s0 + s.n) s = load_seq(bt, ++b, p.page);
+    if (r < s.s0 || r >= s.s0 + s.n) { ++r; continue; }   // a row of no sequence
+    if (!s.ok) {
+      if (lane == 0) report(kErrBadArgument);
+      r = s.s0 + s.n;
+      continue;
+    }
+    const int64_t pos = s.len - s.n + (r - s.s0);
+    const int a = static_cast<int>(pos % BT);             // place of row r in its block
+    if (a != 0 && r != s.s0) {                            // led by an earlier row
+      r = min(r + BT - a, s.s0 + s.n);
+      continue;
+    }
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(BT - a), s.s0 + s.n - r));
+    const int64_t blk = block_index(p, bt, b, pos, h);
+    if (blk < 0) {
+      if (lane == 0) report(kErrBadArgument);
+      r += cnt;
+      continue;
+    }
+    uint32_t x[BT][4];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int t = 0; t < BT; ++t) {
+      if (t < cnt) {
+        load4<X>(src, r + t, h, lane, vec, x[t]);
+      } else {
+        x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0u;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < BT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = max(mx, x[t][i] & 0x7FFFFFFFu);
+    uint32_t E = __reduce_max_sync(0xffffffffu, mx) >> 23;
+    uint32_t* row = reinterpret_cast<uint32_t*>(codes + blk * (BT * HD)) + lane;
+    if (a > 0) {
+      const uint32_t Eo = exps[blk];
+      if (Eo >= E) {
+        E = Eo;
+      } else {
+        const int d = static_cast<int>(E - Eo);
+        for (int t = 0; t < a; ++t) {
+          const uint32_t u = row[t * (HD / 4)];
+          row[t * (HD / 4)] = shift_code(u & 255u, d) | (shift_code(u >> 8 & 255u, d) << 8) |
+                              (shift_code(u >> 16 & 255u, d) << 16) | (shift_code(u >> 24, d) << 24);
+        }
+      }
+      __syncwarp();   // every lane has read the exponent before lane 0 replaces it
+    }
+    if (E >= 7u && E < 255u) {
+      // rint_half_even(x * 2^(133 - E)) by one FMA against 1.5 * 2^23, clamped to the code range
+      constexpr float kMagic = 12582912.0f;
+      const float sc = __uint_as_float((260u - E) << 23);
+#pragma unroll
+      for (int t = 0; t < BT; ++t) {
+        if (t < cnt) {
+          uint32_t u = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float m = fminf(fmaxf(__fsub_rn(fmaf(__uint_as_float(x[t][i]), sc, kMagic), kMagic), -128.0f), 127.0f);
+            u |= (__float_as_uint(__fadd_rn(m, kMagic + 128.0f)) & 0xFFu) << (8 * i);
+          }
+          row[(a + t) * (HD / 4)] = u;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < BT; ++t) {
+        if (t < cnt) {
+          uint32_t u = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u |= static_cast<uint32_t>(bfp16_quant_one(x[t][i], E) + 128) << (8 * i);
+          row[(a + t) * (HD / 4)] = u;
+        }
+      }
+    }
+    if (lane == 0) exps[blk] = static_cast<uint8_t>(E);
+    r += cnt;
+  }
+}
+
+// One thread per 8 values of the output (B, count, Hkv, 128): token start[b] + i of sequence b, zero at and after its
+// length (and on a bad page, which is reported).
+__global__ void __launch_bounds__(256) read_kernel(const Pool p, const int32_t* table, int64_t ld, const int32_t* kv_len,
+                                                   const int32_t* start, int B, int64_t count, uint16_t* ko, uint16_t* vo) {
+  const int64_t per = count * p.hkv * (HD / 8);
+  const int64_t total = per * B;
+  Batch bt{table, ld, kv_len, nullptr, B, 0};
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int b = static_cast<int>(i / per);
+    const int64_t rem = i - b * per;
+    const int64_t tok = rem / (p.hkv * (HD / 8));
+    const int h = static_cast<int>(rem / (HD / 8) % p.hkv), c = static_cast<int>(rem % (HD / 8));
+    const int64_t pos = __ldg(start + b) + tok;
+    const int64_t len = __ldg(kv_len + b);
+    uint32_t wk[4] = {0, 0, 0, 0}, wv[4] = {0, 0, 0, 0};
+    if (pos >= 0 && pos < len) {
+      const int64_t blk = pos < ld * p.page ? block_index(p, bt, b, pos, h) : -1;
+      if (blk < 0) {
+        report(kErrBadArgument);
+      } else {
+        const int64_t off = blk * (BT * HD) + (pos % BT) * HD + c * 8;
+        const uint2 uk = *reinterpret_cast<const uint2*>(p.k + off), uv = *reinterpret_cast<const uint2*>(p.v + off);
+        const uint32_t ek = p.ke[blk], ev = p.ve[blk];
+        bfp16_decode_block_ob(ek, uk.x, uk.y, wk);
+        bfp16_decode_block_ob(ev, uv.x, uv.y, wv);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (ek == 255u) wk[q] = 0x7FC07FC0u;
+          if (ev == 255u) wv[q] = 0x7FC07FC0u;
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(ko + i * 8) = make_uint4(wk[0], wk[1], wk[2], wk[3]);
+    *reinterpret_cast<uint4*>(vo + i * 8) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+  }
+}
+
+// Page pairs travel as a kernel argument: no host-to-device copy, and nothing that the caller has to keep alive.
+template <int N>
+struct Pairs {
+  int32_t src[N], dst[N];
+};
+
+constexpr int kPiece = 16384;   // bytes of a page that one CTA copies: 256 threads x 4 loads of 16 bytes in flight
+
+template <int N>
+__global__ void __launch_bounds__(256) copy_kernel(const Pool p, int64_t layer_codes, int64_t layer_exps,
+                                                   const __grid_constant__ Pairs<N> pairs) {
+  const int64_t bytes = static_cast<int64_t>(p.hkv) * p.page * HD;
+  const int ne = p.hkv * p.page / BT;
+  const int piece = blockIdx.x >> 1;
+  const bool is_v = blockIdx.x & 1;
+  const int64_t src = pairs.src[blockIdx.y], dst = pairs.dst[blockIdx.y];
+  uint8_t* codes = (is_v ? p.v : p.k) + blockIdx.z * layer_codes;
+  const uint4* s = reinterpret_cast<const uint4*>(codes + src * bytes);
+  uint4* d = reinterpret_cast<uint4*>(codes + dst * bytes);
+  const int64_t n16 = bytes / 16;
+  uint4 r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t i = static_cast<int64_t>(piece) * (kPiece / 16) + j * 256 + threadIdx.x;
+    if (i < n16) r[j] = __ldcs(s + i);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t i = static_cast<int64_t>(piece) * (kPiece / 16) + j * 256 + threadIdx.x;
+    if (i < n16) __stcs(d + i, r[j]);
+  }
+  if (piece == 0) {
+    uint8_t* e = (is_v ? p.ve : p.ke) + blockIdx.z * layer_exps;
+    for (int i = threadIdx.x; i < ne; i += 256) e[dst * ne + i] = e[src * ne + i];
+  }
+}
+
+inline int check_pool(const char* fn, const Pool& p) {
+  RL_REQUIRE(p.k && p.v && p.ke && p.ve, RL_ERR_ARGUMENT, "%s: NULL pool pointer", fn);
+  RL_REQUIRE(p.hkv > 0 && p.hkv <= 65535 && p.pages > 0 && p.pages <= INT32_MAX, RL_ERR_ARGUMENT,
+             "%s: need kv_heads >= 1 and 1 <= pages < 2^31", fn);
+  RL_REQUIRE(p.page == 16 || p.page == 32 || p.page == 64 || p.page == 128 || p.page == 256, RL_ERR_ARGUMENT,
+             "%s: page size %d (16, 32, 64, 128 or 256 tokens)", fn, p.page);
+  RL_REQUIRE(aligned(p.k, 16) && aligned(p.v, 16), RL_ERR_ALIGNMENT, "%s: the pool must be 16-byte aligned", fn);
+  return RL_OK;
+}
+
+inline int check_batch(const char* fn, const Batch& bt) {
+  RL_REQUIRE(bt.table && bt.kv_len, RL_ERR_ARGUMENT, "%s: NULL table or kv_len", fn);
+  RL_REQUIRE(bt.B >= 0 && bt.B <= kMaxBatch, RL_ERR_ARGUMENT, "%s: %d sequences (at most %d)", fn, bt.B, kMaxBatch);
+  RL_REQUIRE(bt.ld > 0 && bt.ld <= (1 << 24), RL_ERR_ARGUMENT, "%s: page table of %lld columns", fn, (long long)bt.ld);
+  RL_REQUIRE(bt.T >= 0 && bt.T <= (1 << 24), RL_ERR_ARGUMENT, "%s: %lld rows", fn, (long long)bt.T);
+  RL_REQUIRE(aligned(bt.table, 4) && aligned(bt.kv_len, 4) && aligned(bt.q_start, 4), RL_ERR_ALIGNMENT,
+             "%s: int32 arrays must be 4-byte aligned", fn);
+  return RL_OK;
+}
+
+template <int N>
+inline int copy_launch(const Pool& p, int layers, int64_t lc, int64_t le, const int32_t* src, const int32_t* dst, int n,
+                       cudaStream_t s) {
+  Pairs<N> a;
+  for (int i = 0; i < N; ++i) a.src[i] = i < n ? src[i] : 0, a.dst[i] = i < n ? dst[i] : 0;
+  const int64_t bytes = static_cast<int64_t>(p.hkv) * p.page * HD;
+  const dim3 grid(static_cast<unsigned>((bytes + kPiece - 1) / kPiece * 2), static_cast<unsigned>(n),
+                  static_cast<unsigned>(layers));
+  copy_kernel<N><<<grid, 256, 0, s>>>(p, lc, le, a);
+  RL_TRY_CUDA(cudaGetLastError());
+  return RL_OK;
+}
+
+}  // namespace kv
+}  // namespace rl
+
+extern "C" {
+
+int rl_kv_append(const void* k, int64_t k_st, int64_t k_sh, int64_t k_sd, const void* v, int64_t v_st, int64_t v_sh,
+                 int64_t v_sd, int dtype, int64_t T, uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke,
+                 uint8_t* pool_ve, int64_t pages, int kv_heads, int page, const int32_t* table, int64_t table_ld,
+                 const int32_t* kv_len, const int32_t* q_start, int B, rl_stream_t stream) {
+  using namespace rl;
+  const kv::Pool p{pool_k, pool_v, pool_ke, pool_ve, pages, kv_heads, page};
+  const kv::Batch bt{table, table_ld, kv_len, q_start, B, T};
+  int st;
+  if ((st = kv::check_pool("rl_kv_append", p)) != RL_OK || (st = kv::check_batch("rl_kv_append", bt)) != RL_OK) return st;
+  RL_REQUIRE(dtype == RL_F32 || dtype == RL_BF16, RL_ERR_ARGUMENT, "rl_kv_append: unknown dtype %d", dtype);
+  if (T == 0 || B == 0) return RL_OK;
+  RL_REQUIRE(k && v && q_start, RL_ERR_ARGUMENT, "rl_kv_append: NULL pointer");
+  const uintptr_t es = dtype == RL_F32 ? 4 : 2;
+  RL_REQUIRE(aligned(k, es) && aligned(v, es), RL_ERR_ALIGNMENT, "rl_kv_append: k and v must be aligned to their type");
+  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_append: needs an sm_100 device");
+  // one row per warp while all warps are resident at once (a decode step: every row leads a block of its own), else
+  // 16 rows per warp, of which one or two lead
+  const int rows = T * kv_heads * 2 <= static_cast<int64_t>(sm_count()) * 64 ? 1 : 16;
+  const int64_t groups = (T + rows - 1) / rows;
+  const int64_t ctas = (groups * kv_heads * 2 + 3) / 4;
+  const kv::Source sk{k, k_st, k_sh, k_sd}, sv{v, v_st, v_sh, v_sd};
+  if (dtype == RL_BF16)
+    kv::append_kernel<uint16_t><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
+  else
+    kv::append_kernel<float><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
+  RL_TRY_CUDA(cudaGetLastError());
+  return RL_OK;
+}
+
+int rl_kv_read(const uint8_t* pool_k, const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve,
+               int64_t pages, int kv_heads, int page, const int32_t* table, int64_t table_ld, const int32_t* kv_len,
+               const int32_t* start, int B, int64_t count, uint16_t* k_out, uint16_t* v_out, rl_stream_t stream) {
+  using namespace rl;
+  const kv::Pool p{const_cast<uint8_t*>(pool_k), const_cast<uint8_t*>(pool_v), const_cast<uint8_t*>(pool_ke),
+                   const_cast<uint8_t*>(pool_ve), pages, kv_heads, page};
+  const kv::Batch bt{table, table_ld, kv_len, nullptr, B, 0};
+  int st;
+  if ((st = kv::check_pool("rl_kv_read", p)) != RL_OK || (st = kv::check_batch("rl_kv_read", bt)) != RL_OK) return st;
+  RL_REQUIRE(count >= 0 && count <= (1 << 28), RL_ERR_ARGUMENT, "rl_kv_read: count %lld", (long long)count);
+  if (count == 0 || B == 0) return RL_OK;
+  RL_REQUIRE(start && k_out && v_out, RL_ERR_ARGUMENT, "rl_kv_read: NULL pointer");
+  RL_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(start, 4), RL_ERR_ALIGNMENT,
+             "rl_kv_read: outputs must be 16-byte aligned");
+  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_read: needs an sm_100 device");
+  const int64_t work = static_cast<int64_t>(B) * count * kv_heads * (kv::HD / 8);
+  const int64_t ctas = (work + 255) / 256, most = static_cast<int64_t>(sm_count()) * 64;
+  kv::read_kernel<<<static_cast<unsigned>(ctas < most ? ctas : most), 256, 0, stream>>>(p, table, table_ld, kv_len,
+                                                                                         start, B, count, k_out, v_out);
+  RL_TRY_CUDA(cudaGetLastError());
+  return RL_OK;
+}
+
+int rl_kv_copy_pages(uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke, uint8_t* pool_ve, int layers, int64_t pages,
+                     int kv_heads, int page, const int32_t* src, const int32_t* dst, int64_t n, rl_stream_t stream) {
+  using namespace rl;
+  const kv::Pool p{pool_k, pool_v, pool_ke, pool_ve, pages, kv_heads, page};
+  int st;
+  if ((st = kv::check_pool("rl_kv_copy_pages", p)) != RL_OK) return st;
+  RL_REQUIRE(layers > 0 && layers <= 65535, RL_ERR_ARGUMENT, "rl_kv_copy_pages: %d layers", layers);
+  RL_REQUIRE(n >= 0 && n <= pages, RL_ERR_ARGUMENT, "rl_kv_copy_pages: %lld copies in %lld pages", (long long)n,
+             (long long)pages);
+  if (n == 0) return RL_OK;
+  RL_REQUIRE(src && dst, RL_ERR_ARGUMENT, "rl_kv_copy_pages: NULL pointer");
+  // The copies of one call run at once: a page may be copied to several others, but a page that is written must be
+  // neither read nor written by another copy.
+  uint8_t* seen = static_cast<uint8_t*>(std::calloc(static_cast<size_t>(pages), 1));
+  RL_REQUIRE(seen, RL_ERR_ARGUMENT, "rl_kv_copy_pages: out of host memory");
+  int64_t bad = -1;
+  for (int64_t i = 0; i < n && bad < 0; ++i) {
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages || (seen[dst[i]] & 1)) bad = i;
+    else seen[dst[i]] |= 1;
+  }
+  for (int64_t i = 0; i < n && bad < 0; ++i)
+    if (seen[src[i]] & 1) bad = i;
+  std::free(seen);
+  RL_REQUIRE(bad < 0, RL_ERR_ARGUMENT,
+             "rl_kv_copy_pages: copy %lld (page %d to %d): pages lie in [0, %lld), and a page that is written is neither "
+             "read nor written by another copy of the call", (long long)bad, src[bad], dst[bad], (long long)pages);
+  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_copy_pages: needs an sm_100 device");
+  const int64_t le = pages * kv_heads * (page / kv::BT), lc = pages * kv_heads * page * kv::HD;
+  for (int64_t i = 0; i < n; i += 1024) {
+    const int m = static_cast<int>(n - i < 1024 ? n - i : 1024);
+    st = m <= 32 ? kv::copy_launch<32>(p, layers, lc, le, src + i, dst + i, m, stream)
+                 : kv::copy_launch<1024>(p, layers, lc, le, src + i, dst + i, m, stream);
+    if (st != RL_OK) return st;
+  }
+  return RL_OK;
+}
+
+}  // extern "C"

@@ -9,6 +9,11 @@ through its C ABI on the current torch stream.
   PackedWeight     a packed B operand resident on the GPU (native tile order)
   linear_bfp16     gemm() / matmul_vectorized_bfp16 (+ bias)      redline/forward.py:194-197
   swiglu_up        matmul_swiglu_bfp16 (up GEMM + SwiGLU flush)   kernels/atb3/mm_bfp_swiglu.cc:88-168
+
+Continuing sequences token by token (no counterpart in the reference):
+
+  KVPool, kv_append, kv_read, kv_copy_pages, kv_attention   the 8-bit paged cache (cache.PagedKV manages its pages)
+  Weight4, linear_w4, swiglu_w4                             products of up to 64 rows with 4-bit weights
 """
 
 import torch
@@ -298,6 +303,210 @@ def conv2d(x_dq, w, bias, taps, out=None):
     L.call("rl_conv2d_bfp16", _ptr(x_dq), H, Wd, C, _ptr(w.native), w.N, taps, _ptr(bias), _ptr(out), _ptr(ws),
            ws.numel(), _stream())
     return out
+
+
+def _check_here(*ts):
+    """CUDA tensors of the current device (any strides)."""
+    dev = None
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError("redline_tiny_b200 ops take CUDA tensors (no CPU path)")
+            if dev is None:
+                dev = torch.cuda.current_device()
+            if t.device.index != dev:
+                raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+
+
+def _check_int32(name, t, shape):
+    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be contiguous int32 of shape {shape}, not {t.dtype} {tuple(t.shape)}")
+
+
+KV_BLOCK = 16   # tokens of one K/V head that share an exponent
+
+
+class KVPool:
+    """The pages of an 8-bit cache: k, v uint8 (layers, pages, kv_heads, page, 128) and k_exp, v_exp uint8
+    (layers, pages, kv_heads, page / 16). A block of 16 tokens of one head shares one exponent:
+    value = (k - 128) * 2^(k_exp - 133); exponent 255 reads as NaN."""
+
+    def __init__(self, k, v, k_exp, v_exp):
+        _check_here(k, v, k_exp, v_exp)
+        if k.dim() != 5 or k.shape[4] != 128 or k.shape[3] not in (16, 32, 64, 128, 256):
+            raise ValueError("cache codes must be (layers, pages, kv_heads, page, 128), page = 16, 32, 64, 128 or 256")
+        exps = (*k.shape[:3], k.shape[3] // KV_BLOCK)
+        for t, shape in ((k, k.shape), (v, k.shape), (k_exp, exps), (v_exp, exps)):
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.shape != shape:
+                raise ValueError(f"cache tensors must be contiguous uint8; expected {tuple(shape)}, got {tuple(t.shape)}")
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self.layers, self.pages, self.kv_heads, self.page = k.shape[:4]
+        self._ptrs = [tuple(t[i].data_ptr() for t in (k, v, k_exp, v_exp)) for i in range(self.layers)]
+
+    @classmethod
+    def empty(cls, layers, pages, kv_heads, page=64, device="cuda"):
+        codes = (layers, pages, kv_heads, page, 128)
+        exps = (layers, pages, kv_heads, page // KV_BLOCK)
+        return cls(*[torch.full(s, f, dtype=torch.uint8, device=device) for s, f in
+                     ((codes, 128), (codes, 128), (exps, 0), (exps, 0))])
+
+    def _args(self, layer):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of a cache with {self.layers}")
+        return (*self._ptrs[layer], self.pages, self.kv_heads, self.page)
+
+
+def _batch(pool, table, kv_len, q_start=None):
+    _check_here(pool.k, table, kv_len, q_start)
+    if table.dim() != 2 or table.shape[1] == 0:
+        raise ValueError("table must be int32 (sequences, pages)")
+    B = table.shape[0]
+    _check_int32("table", table, (B, table.shape[1]))
+    _check_int32("kv_len", kv_len, (B,))
+    if q_start is not None:
+        _check_int32("q_start", q_start, (B + 1,))
+    return B
+
+
+def kv_append(pool, layer, k, v, table, kv_len, q_start):
+    """Write the keys and values of new tokens, k, v (T, kv_heads, 128) bf16 or fp32 of any strides, into a layer of the
+    cache. table int32 (B, pages), kv_len int32 (B) with the new tokens counted, q_start int32 (B + 1): the new tokens
+    of sequence b are rows q_start[b] .. q_start[b + 1] - 1 and take its last positions. A block's exponent grows to
+    hold them, and older codes of the block are shifted. The pages written must belong to one sequence each."""
+    B = _batch(pool, table, kv_len, q_start)
+    _check_here(pool.k, k, v)
+    if k.dim() != 3 or tuple(k.shape[1:]) != (pool.kv_heads, 128) or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k and v must be (rows, {pool.kv_heads}, 128) of one dtype")
+    L.call("rl_kv_append", _ptr(k), *k.stride(), _ptr(v), *v.stride(), _dtype_code(k), k.shape[0], *pool._args(layer),
+           _ptr(table), table.shape[1], _ptr(kv_len), _ptr(q_start), B, _stream())
+
+
+def kv_read(pool, layer, table, kv_len, start, count):
+    """Positions start[b] .. start[b] + count - 1 of each sequence of a layer as (k, v) bf16 (B, count, kv_heads, 128),
+    exactly; zeros at and after kv_len[b]."""
+    B = _batch(pool, table, kv_len)
+    _check_here(pool.k, start)
+    _check_int32("start", start, (B,))
+    k = torch.empty((B, int(count), pool.kv_heads, 128), dtype=torch.bfloat16, device=pool.k.device)
+    v = torch.empty_like(k)
+    L.call("rl_kv_read", *pool._args(layer), _ptr(table), table.shape[1], _ptr(kv_len), _ptr(start), B, int(count),
+           _ptr(k), _ptr(v), _stream())
+    return k, v
+
+
+def kv_copy_pages(pool, src, dst):
+    """Copy page src[i] to page dst[i] in every layer (src, dst: sequences of ints on the host). The copies run at once:
+    a page that is written is neither read nor written by another copy of the call."""
+    import array
+    _check_here(pool.k)
+    a, b = array.array("i", src), array.array("i", dst)
+    if len(a) != len(b):
+        raise ValueError(f"{len(a)} source pages for {len(b)} destinations")
+    L.call("rl_kv_copy_pages", *pool._ptrs[0], pool.layers, pool.pages, pool.kv_heads, pool.page, a.buffer_info()[0],
+           b.buffer_info()[0], len(a), _stream())
+
+
+def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_log2=None, out=None):
+    """Attention of new tokens q (T, heads, 128) bf16 (any row and head strides that are multiples of 8) over a layer of
+    the cache, which holds their own keys already (kv_append). Row j of sequence b's n new rows sees positions
+    <= kv_len[b] - n + j, or <= min(row_limit[row], kv_len[b] - 1) with row_limit int32 (T); a row that sees no key gives
+    zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128). scale_log2 defaults to
+    log2(e)/sqrt(128)."""
+    B = _batch(pool, table, kv_len, q_start)
+    _check_here(pool.k, q, row_limit, out)
+    if q.dim() != 3 or q.shape[2] != 128 or q.stride(2) != 1 or q.dtype != torch.bfloat16:
+        raise ValueError("q must be bf16 (rows, heads, 128) with contiguous head vectors")
+    T, H = q.shape[:2]
+    if row_limit is not None:
+        _check_int32("row_limit", row_limit, (T,))
+    if out is None:
+        out = torch.empty((T, H * 128), dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, H * 128) or (T and out.stride(1) != 1):
+        raise ValueError(f"out must be bf16 ({T}, {H * 128}) with contiguous rows")
+    ws = torch.empty(max(L.lib().rl_kv_attention_workspace(T, B, H, pool.kv_heads), 16), dtype=torch.uint8,
+                     device=q.device)
+    L.call("rl_kv_attention", _ptr(q), q.stride(0), q.stride(1), T, H, *pool._args(layer), _ptr(table), table.shape[1],
+           _ptr(kv_len), _ptr(q_start), B, _ptr(row_limit), _SCALE_LOG2 if scale_log2 is None else float(scale_log2),
+           _ptr(out), out.stride(0), _ptr(ws), ws.numel(), _stream())
+    return out
+
+
+_SCALE_LOG2 = 1.4426950408889634 / 128 ** 0.5
+
+
+class Weight4:
+    """A B operand (K, N) in 4 bits with a bf16 scale per `group` values of a column, resident on the GPU in the native
+    order: value (u - 8) * s. swiglu=True marks an up matrix with [gate 64 | proj 64] per 128 columns, as PackedWeight."""
+
+    def __init__(self, codes, scales, K, N, group, swiglu=False):
+        self.codes, self.scales = codes, scales
+        self.K, self.N, self.group, self.swiglu = int(K), int(N), int(group), bool(swiglu)
+
+    @classmethod
+    def from_codes(cls, codes, scales, swiglu=False):
+        """codes uint8 (K, N), one value 0 .. 15 per byte, and scales bf16 (K / group, N) -> native order."""
+        import ctypes
+        _check_here(codes, scales)
+        _check_cuda(codes, scales)
+        K, N = codes.shape
+        if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or scales.shape[1] != N or \
+                scales.shape[0] == 0 or K % scales.shape[0]:
+            raise ValueError("codes must be uint8 (K, N) and scales bf16 (K / group, N)")
+        group = K // scales.shape[0]
+        nb = [ctypes.c_size_t(), ctypes.c_size_t()]
+        L.call("rl_w4_bytes", K, N, group, int(swiglu), *[ctypes.byref(b) for b in nb])
+        w, s = (torch.empty(b.value, dtype=torch.uint8, device=codes.device) for b in nb)
+        L.call("rl_w4_pack", _ptr(codes), _ptr(scales), K, N, group, int(swiglu), _ptr(w), _ptr(s), _stream())
+        return cls(w, s, K, N, group, swiglu)
+
+    @classmethod
+    def from_float(cls, B, group=64, swiglu=False):
+        """Float B (K, N) on the GPU, rounded to 4 bits there."""
+        return cls.from_codes(*quantize_w4(B, group), swiglu=swiglu)
+
+
+def quantize_w4(B, group=64):
+    """B (K, N) fp32/bf16 -> (codes uint8 (K, N), scales bf16 (K / group, N)): s = bf16(e / -8) with e the group's value
+    of largest magnitude, u = clip(rint(w / s) + 8, 0, 15)."""
+    _check_here(B)
+    _check_cuda(B)
+    K, N = B.shape
+    codes = torch.empty((K, N), dtype=torch.uint8, device=B.device)
+    scales = torch.empty((K // max(int(group), 1), N), dtype=torch.bfloat16, device=B.device)
+    L.call("rl_w4_quantize", _ptr(B), _dtype_code(B), K, N, int(group), _ptr(codes), _ptr(scales), _stream())
+    return codes, scales
+
+
+def _w4(x, w, bias, epi, out, cols, out_dtype):
+    _check_here(x, w.codes, bias, out)
+    _check_cuda(x, bias, out)
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != w.K:
+        raise ValueError(f"x must be bf16 (rows, {w.K}), not {x.dtype} {tuple(x.shape)}")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (w.N,)):
+        raise ValueError(f"bias must be bf16 ({w.N},)")
+    if out is None:
+        out = torch.empty((x.shape[0], cols), dtype=out_dtype, device=x.device)
+    elif tuple(out.shape) != (x.shape[0], cols):
+        raise ValueError(f"out must be {(x.shape[0], cols)}")
+    L.call("rl_linear_w4", _ptr(x), x.shape[0], w.K, _ptr(w.codes), _ptr(w.scales), w.N, w.group, _ptr(bias), epi,
+           _ptr(out), _dtype_code(out), _stream())
+    return out
+
+
+def linear_w4(x, w, bias=None, out=None, out_dtype=torch.bfloat16):
+    """C = x @ B (+ bias) for up to 64 rows x (M, K) bf16 (any bf16 values) and a Weight4: the products of a decode step
+    (linear_bfp16 takes more rows)."""
+    if w.swiglu:
+        raise ValueError("linear_w4 takes a Weight4 packed without swiglu (swiglu_w4 takes the others)")
+    return _w4(x, w, bias, L.RL_EPI_NONE if bias is None else L.RL_EPI_BIAS, out, w.N, out_dtype)
+
+
+def swiglu_w4(x, w_up, bias=None, out=None, out_dtype=torch.bfloat16):
+    """H = silu(x @ Bgate) * (x @ Bproj) for up to 64 rows, bf16 (M, N / 2) rounded once (not to bfp16 blocks: linear_w4
+    takes any bf16 values). w_up must be packed with swiglu=True."""
+    if not w_up.swiglu:
+        raise ValueError("swiglu_w4 needs a Weight4 packed with swiglu=True")
+    return _w4(x, w_up, bias, L.RL_EPI_SWIGLU, out, w_up.N // 2, out_dtype)
 
 
 def set_gemm_variant(v):
