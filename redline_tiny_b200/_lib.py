@@ -112,7 +112,7 @@ def lib():
 
 def call(name, *args):
     """Call a C-ABI entry point; raise RedlineError on a non-zero status."""
-    st = getattr(lib(), name)(*args)
+    st = getattr(_lib or lib(), name)(*args)
     if st != RL_OK:
         raise RedlineError(name, st, lib().rl_last_error().decode(errors="replace"))
     return st

@@ -87,6 +87,20 @@ __device__ __forceinline__ uint32_t codes_h2(uint32_t w) {
   return h2sub(__byte_perm(w, 0x64646464u, kSel), 0x64806480u);
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+
 // The list of units: sequence b has hkv * tiles(b) tasks of chunks(b) units each.
 __device__ __forceinline__ int64_t tiles_of(const Args& a, const kv::Seq& s, int R) {
   return (s.n * a.group + R - 1) / R;
@@ -130,7 +144,7 @@ struct Acc {
 // One warp, one block of 16 keys starting at position pos0.
 template <int NT>
 __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&vr)[4], uint32_t ke, uint32_t ve,
-                                           int64_t pos0, const uint32_t (&qf)[NT][16], const float (&qs)[NT][2],
+                                           int64_t pos0, const uint32_t (&qf)[16], uint32_t q_at, const float (&qs)[NT][2],
                                            const int (&lim)[NT][2], int lim_min, int g, Acc<NT>& acc) {
   float s[NT][4];
 #pragma unroll
@@ -138,12 +152,22 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
   const uint32_t* k0[2] = {&kr[0].x, &kr[1].x};   // token g: dims 16c.., 64 + 16c..
   const uint32_t* k1[2] = {&kr[2].x, &kr[3].x};   // token g + 8
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t w0 = k0[j >> 2][j & 3], w1 = k1[j >> 2][j & 3];
-    const uint32_t a0 = codes_h2<0x4140>(w0), a2 = codes_h2<0x4342>(w0);
-    const uint32_t a1 = codes_h2<0x4140>(w1), a3 = codes_h2<0x4342>(w1);
+  for (int jj = 0; jj < 4; ++jj) {
+    uint32_t A[2][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) mma(s[nt], a0, a1, a2, a3, qf[nt][2 * j], qf[nt][2 * j + 1]);
+    for (int i = 0; i < 2; ++i) {
+      const int j = 2 * jj + i;
+      const uint32_t w0 = k0[j >> 2][j & 3], w1 = k1[j >> 2][j & 3];
+      A[i][0] = codes_h2<0x4140>(w0), A[i][2] = codes_h2<0x4342>(w0);
+      A[i][1] = codes_h2<0x4140>(w1), A[i][3] = codes_h2<0x4342>(w1);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint4 q = make_uint4(qf[4 * jj], qf[4 * jj + 1], qf[4 * jj + 2], qf[4 * jj + 3]);
+      if (NT > 1) q = lds128(q_at + (nt * 4 + jj) * 512);
+      mma(s[nt], A[0][0], A[0][1], A[0][2], A[0][3], q.x, q.y);
+      mma(s[nt], A[1][0], A[1][1], A[1][2], A[1][3], q.z, q.w);
+    }
   }
   const float ks = ke == 255u ? __uint_as_float(0x7FC00000u) : bfp16_scale(ke);
   bool raise = false;
@@ -223,21 +247,35 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
   }
 }
 
+// Shared memory of a CTA: the ring that brings blocks in (per warp kStages x [K 2 KB | V 2 KB]), reused at the end of a
+// run for the warps' results (kWarps x R x 128 floats), then their maxima and sums, then the unit prefix.
 template <int NT>
-__device__ __forceinline__ int64_t smem_floats() { return static_cast<int64_t>(kWarps) * 8 * NT * (HD + 2); }
+struct Cfg {
+  static constexpr int R = 8 * NT;
+  static constexpr int kStages = NT == 4 ? 4 : 3;
+  static constexpr int kCtas = NT == 1 ? 4 : 2;                       // resident per SM
+  static constexpr int kRing = kWarps * kStages * 2 * BT * HD;
+  static constexpr int kOut = kWarps * R * HD * 4;
+  static constexpr int kBody = kRing > kOut ? kRing : kOut;
+  static constexpr int kQ = NT == 1 ? 0 : NT * 16 * 32 * 4;            // q fragments, where registers cannot hold them
+  static size_t smem(int B) { return kBody + kQ + kWarps * R * 8 + (kWarps + B + 1) * sizeof(int64_t); }
+};
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const Args a) {
   constexpr int R = 8 * NT;
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int S = Cfg<NT>::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
   float* so = reinterpret_cast<float*>(smem);                        // [warp][row][128]
-  float* sm = so + kWarps * R * HD;                                  // [warp][row] maxima
+  uint8_t* sq = smem + Cfg<NT>::kBody;                               // [n-tile][4][lane] x 16 bytes
+  float* sm = reinterpret_cast<float*>(sq + Cfg<NT>::kQ);            // [warp][row] maxima
   float* sl = sm + kWarps * R;                                       // [warp][row] sums
   int64_t* warp_sum = reinterpret_cast<int64_t*>(sl + kWarps * R);
   int64_t* pre = warp_sum + kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   unit_prefix(a, R, pre, warp_sum);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t U = pre[a.batch.B];
   const int64_t C = min(static_cast<int64_t>(gridDim.x), U);        // every working CTA has at least one unit
   const bool idle = blockIdx.x >= C;
@@ -246,6 +284,14 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
   bool first = true;
   Piece rec{0, 0, 0, 0};
   int b = 0;
+
+  // ring addresses of this lane. Row r of a block keeps its 16-byte chunk j at chunk j ^ f(r), f = 4 (r & 1) for K and
+  // 2 ((r >> 1) & 3) for V, so that the eight lanes of a shared-memory phase read eight different bank groups.
+  const uint32_t ring = smem_u32(smem) + warp * (S * 2 * BT * HD);
+  const int wr = lane >> 3, wc = lane & 7;                           // copies: rows wr, wr + 4, ..; chunk wc
+  const uint32_t k_ld = g * HD + ((c ^ ((g & 1) * 4)) << 4);
+  const uint32_t v_ld = BT * HD + 2 * c * HD + ((g ^ (2 * c)) << 4);
+
   while (u < u_end) {
     // the task of unit u
     int lo = b, hi = a.batch.B;
@@ -262,34 +308,14 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     const int64_t tile = task / a.pool.hkv;
     const int64_t rows = s.n * a.group;                              // rows of this K/V head
 
-    uint32_t qf[NT][16];
+    uint32_t qf[16];
     float qs[NT][2];
     int lim[NT][2];
     int lim_min = INT32_MAX, lim_max = -1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int64_t r = tile * R + nt * 8 + g;                       // the row whose q this lane loads
-      uint4 w[4] = {};
-      if (r < rows) {
-        const uint16_t* p = a.q + (s.s0 + r / a.group) * a.q_st + (h * a.group + r % a.group) * a.q_sh + 16 * c;
-        w[0] = *reinterpret_cast<const uint4*>(p), w[1] = *reinterpret_cast<const uint4*>(p + 8);
-        w[2] = *reinterpret_cast<const uint4*>(p + 64), w[3] = *reinterpret_cast<const uint4*>(p + 72);
-      }
-      const uint32_t* x = &w[0].x;
-      uint32_t mx = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = max(mx, max(x[i] & 0x7FFFu, x[i] >> 16 & 0x7FFFu));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const uint32_t e = max(mx >> 7, 32u);                          // exponent field (values below 2^-95 keep less)
-      const float up = __uint_as_float((268u - e) << 23);            // 2^(141 - e)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        qf[nt][i] = pack_h2(__uint_as_float(x[i] << 16) * up, __uint_as_float(x[i] & 0xFFFF0000u) * up);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int ec = __shfl_sync(0xffffffffu, static_cast<int>(e), (2 * c + k) * 4);
-        qs[nt][k] = __uint_as_float(static_cast<uint32_t>(ec - 14) << 23) * a.scale_log2;   // 2^(e - 141)
         const int64_t rr = tile * R + nt * 8 + 2 * c + k;
         int64_t L = -1;
         if (rr < rows) {
@@ -306,6 +332,81 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
 
+    // the warp's blocks: every fourth of the run. Lane j holds the pool index of block 32 t + j, one chunk ahead.
+    const int64_t key_end = min(ch1 * UNIT, static_cast<int64_t>(lim_max) + 1);
+    const int64_t pos0 = ch0 * UNIT + warp * BT;
+    const int n = key_end > pos0 ? static_cast<int>((key_end - pos0 + UNIT - 1) / UNIT) : 0;
+    auto block_of = [&](int k) -> int {
+      if (k >= n) return -1;
+      const int64_t blk = kv::block_index(a.pool, a.batch, b, pos0 + static_cast<int64_t>(k) * UNIT, h);
+      if (blk < 0) report(kErrBadArgument);                          // a page outside the pool: its keys are absent
+      return static_cast<int>(blk);
+    };
+    int idx = block_of(lane), idx_next = block_of(32 + lane);
+    uint32_t ex[S];                                                  // ke | ve << 8 | present << 16 of the ring's blocks
+    auto issue = [&](int k, uint32_t& e) {
+      if (k < n) {
+        if ((k & 31) == 0 && k > 0) {
+          idx = idx_next;
+          idx_next = block_of(k + 32 + lane);
+        }
+        const int64_t blk = __shfl_sync(0xffffffffu, idx, k & 31);
+        e = 0;
+        if (blk >= 0) {
+          e = a.pool.ke[blk] | (a.pool.ve[blk] << 8) | 0x10000u;
+          const uint8_t* kp = a.pool.k + blk * (BT * HD) + lane * 16;
+          const uint8_t* vp = a.pool.v + blk * (BT * HD) + lane * 16;
+          const uint32_t d = ring + (k % S) * (2 * BT * HD) + wr * HD;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) cp_async16(d + j * 4 * HD + ((wc ^ ((wr & 1) * 4)) << 4), kp + j * 512);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            cp_async16(d + BT * HD + j * 4 * HD + ((wc ^ ((((wr + 4 * j) >> 1) & 3) * 2)) << 4), vp + j * 512);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k) issue(k, ex[k]);
+
+    // q of the tile, while the first blocks are on their way
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int64_t r = tile * R + nt * 8 + g;                       // the row whose q this lane loads
+      uint4 w[4] = {};
+      if (r < rows) {
+        const uint16_t* p = a.q + (s.s0 + r / a.group) * a.q_st + (h * a.group + r % a.group) * a.q_sh + 16 * c;
+        w[0] = *reinterpret_cast<const uint4*>(p), w[1] = *reinterpret_cast<const uint4*>(p + 8);
+        w[2] = *reinterpret_cast<const uint4*>(p + 64), w[3] = *reinterpret_cast<const uint4*>(p + 72);
+      }
+      const uint32_t x[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
+                              w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = max(mx, max(x[i] & 0x7FFFu, x[i] >> 16 & 0x7FFFu));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const uint32_t e = max(mx >> 7, 32u);                          // exponent field (values below 2^-95 keep less)
+      const float up = __uint_as_float((268u - e) << 23);            // 2^(141 - e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        qf[i] = pack_h2(__uint_as_float(x[i] << 16) * up, __uint_as_float(x[i] & 0xFFFF0000u) * up);
+      if (NT > 1 && nt % kWarps == warp) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          reinterpret_cast<uint4*>(sq)[(nt * 4 + i) * 32 + lane] =
+              make_uint4(qf[4 * i], qf[4 * i + 1], qf[4 * i + 2], qf[4 * i + 3]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int ec = __shfl_sync(0xffffffffu, static_cast<int>(e), (2 * c + k) * 4);
+        qs[nt][k] = __uint_as_float(static_cast<uint32_t>(ec - 14) << 23) * a.scale_log2;   // 2^(e - 141)
+      }
+    }
+
+    if (NT > 1) __syncthreads();
+    const uint32_t q_at = smem_u32(sq) + lane * 16;
+
     Acc<NT> acc;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -314,22 +415,29 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc.o[nt][i][0] = acc.o[nt][i][1] = acc.o[nt][i][2] = acc.o[nt][i][3] = 0.0f;
     }
-    const int64_t key_end = min(ch1 * UNIT, static_cast<int64_t>(lim_max) + 1);
-    for (int64_t pos = ch0 * UNIT + warp * BT; pos < key_end; pos += kWarps * BT) {
-      const int64_t blk = kv::block_index(a.pool, a.batch, b, pos, h);
-      if (blk < 0) {   // a page outside the pool: its keys count as absent
-        if (lane == 0) report(kErrBadArgument);
-        continue;
+    for (int i0 = 0; i0 < n; i0 += S) {
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const int i = i0 + j;
+        if (i < n) {
+          cp_wait<S - 2>();
+          __syncwarp();        // block i of every lane is in; every lane is done with block i - 1
+          issue(i + S - 1, ex[(j + S - 1) % S]);
+          if (ex[j] & 0x10000u) {
+            const uint32_t at = ring + j * (2 * BT * HD);
+            uint4 kr[4], vr[4];
+            kr[0] = lds128(at + k_ld), kr[1] = lds128(at + (k_ld ^ 64));
+            kr[2] = lds128(at + k_ld + 8 * HD), kr[3] = lds128(at + (k_ld ^ 64) + 8 * HD);
+            vr[0] = lds128(at + v_ld), vr[1] = lds128(at + v_ld + HD);
+            vr[2] = lds128(at + v_ld + 8 * HD), vr[3] = lds128(at + v_ld + 9 * HD);
+            block_step<NT>(kr, vr, ex[j] & 255u, ex[j] >> 8 & 255u, pos0 + static_cast<int64_t>(i) * UNIT, qf, q_at, qs, lim,
+                           lim_min, g, acc);
+          }
+        }
       }
-      const uint8_t* kp = a.pool.k + blk * (BT * HD) + g * HD + 16 * c;
-      const uint8_t* vp = a.pool.v + blk * (BT * HD) + 2 * c * HD + 16 * g;
-      uint4 kr[4], vr[4];
-      kr[0] = *reinterpret_cast<const uint4*>(kp), kr[1] = *reinterpret_cast<const uint4*>(kp + 64);
-      kr[2] = *reinterpret_cast<const uint4*>(kp + 8 * HD), kr[3] = *reinterpret_cast<const uint4*>(kp + 8 * HD + 64);
-      vr[0] = *reinterpret_cast<const uint4*>(vp), vr[1] = *reinterpret_cast<const uint4*>(vp + HD);
-      vr[2] = *reinterpret_cast<const uint4*>(vp + 8 * HD), vr[3] = *reinterpret_cast<const uint4*>(vp + 9 * HD);
-      block_step<NT>(kr, vr, a.pool.ke[blk], a.pool.ve[blk], pos, qf, qs, lim, lim_min, g, acc);
     }
+    cp_wait<0>();
+    __syncthreads();           // every warp is done with the ring
 
     // join the warps: (O, m, l) of each through shared memory
 #pragma unroll
@@ -388,33 +496,46 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
   if (threadIdx.x == 0) a.rec[blockIdx.x] = make_int4(rec.b, rec.h, rec.tile, rec.n);
 }
 
-// CTA i joins the pieces of the task that CTA i of attend_kernel began and did not finish.
+// CTA i joins the pieces of the task that CTA i of attend_kernel began and did not finish: a warp per row, 4 dims a lane.
+// Launched while attend_kernel still runs (its CTAs need no more than a slot), it waits for that grid's end.
+constexpr int kJoin = 8;   // warps
 template <int NT>
-__global__ void __launch_bounds__(HD) combine_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * kJoin) combine_kernel(const Args a) {
   constexpr int R = 8 * NT;
+  constexpr int64_t kSlot = R * (HD + 2);
+  const int lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 rec = a.rec[blockIdx.x];
   if (rec.w == 0) return;
   const int pieces = abs(rec.w);
   const kv::Seq s = kv::load_seq(a.batch, rec.x, a.pool.page);
   const int64_t rows = s.n * a.group;
-  const int d = threadIdx.x;
-  for (int row = 0; row < R; ++row) {
+  // piece 0 may lie in the CTA's second slot; the others in the first slots of the CTAs behind
+  const float* base = a.part + static_cast<int64_t>(blockIdx.x) * 2 * kSlot;
+  auto piece = [&](int j) { return base + (j == 0 ? (rec.w < 0 ? kSlot : 0) : j * 2 * kSlot); };
+  for (int row = threadIdx.x >> 5; row < R; row += kJoin) {
     const int64_t r = static_cast<int64_t>(rec.z) * R + row;
     if (r >= rows) break;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    float m = -INFINITY;
+    for (int j = lane; j < pieces; j += 32) m = fmaxf(m, piece(j)[R * HD + row]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float z = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
     for (int j = 0; j < pieces; ++j) {
-      const float* part = a.part + ((static_cast<int64_t>(blockIdx.x) + j) * 2 + (j == 0 && rec.w < 0)) * R * (HD + 2);
-      const float mj = part[R * HD + row];
-      const float mn = fmaxf(m, mj);
-      const float z = mn == -INFINITY ? 0.0f : mn;
-      const float fa = exp2f(m - z), fb = exp2f(mj - z);
-      l = l * fa + part[R * HD + R + row] * fb;
-      o = o * fa + part[row * HD + d] * fb;
-      m = mn;
+      const float* p = piece(j);
+      const float4 v = *reinterpret_cast<const float4*>(p + row * HD + 4 * lane);
+      const float f = exp2f(p[R * HD + row] - z);
+      l = fmaf(f, p[R * HD + R + row], l);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    a.o[(s.s0 + r / a.group) * a.ldo + (rec.y * a.group + r % a.group) * HD + d] =
-        __bfloat16_as_ushort(__float2bfloat16_rn(o * inv));
+    uint16_t* d = a.o + (s.s0 + r / a.group) * a.ldo + (rec.y * a.group + r % a.group) * HD + 4 * lane;
+    const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
   }
 }
 
@@ -424,18 +545,27 @@ inline int tile_n(int64_t T, int B, int group) {
   const int64_t rows = B > 0 ? (T * group + B - 1) / B : 0;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
-inline int ctas_of(int nt) { return sm_count() * (nt == 1 ? 3 : nt == 2 ? 2 : 1); }
+inline int ctas_of(int nt) { return sm_count() * (nt == 1 ? Cfg<1>::kCtas : nt == 2 ? Cfg<2>::kCtas : Cfg<4>::kCtas); }
 inline size_t part_bytes(int nt) { return static_cast<size_t>(ctas_of(nt)) * 2 * 8 * nt * (HD + 2) * 4; }
 
 template <int NT>
 inline int launch(const Args& a, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(kWarps) * 8 * NT * (HD + 2) * 4 + (kWarps + a.batch.B + 1) * sizeof(int64_t);
-  RL_TRY_CUDA(cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  const size_t smem = Cfg<NT>::smem(a.batch.B);
   const int ctas = ctas_of(NT);
+  RL_TRY_CUDA(cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch))));
   attend_kernel<NT><<<ctas, kThreads, smem, st>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
-  combine_kernel<NT><<<ctas, HD, 0, st>>>(a);
-  RL_TRY_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(32 * kJoin);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  RL_TRY_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<NT>, a));
   return RL_OK;
 }
 
@@ -467,6 +597,8 @@ int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, in
     return st;
   RL_REQUIRE(heads > 0 && heads % kv_heads == 0, RL_ERR_ARGUMENT, "rl_kv_attention: %d query heads over %d K/V heads",
              heads, kv_heads);
+  RL_REQUIRE(pages * kv_heads * (page / kv::BT) <= INT32_MAX, RL_ERR_ARGUMENT, "rl_kv_attention: %lld pages",
+             (long long)pages);
   RL_REQUIRE(table_ld * page <= (1 << 30), RL_ERR_ARGUMENT, "rl_kv_attention: sequences of up to %lld tokens",
              (long long)(table_ld * page));
   if (T == 0 || B == 0) return RL_OK;

@@ -16,6 +16,11 @@ Continuing sequences token by token (no counterpart in the reference):
   Weight4, linear_w4, swiglu_w4                             products of up to 64 rows with 4-bit weights
 """
 
+import array
+import ctypes
+import functools
+import math
+
 import torch
 
 from . import _lib as L
@@ -127,7 +132,6 @@ class PackedWeight:
 def weights_shard(K, N, rank, world):
     """(n0, n_cols, byte_offset, byte_count) of column shard `rank` of `world` of a packed B (K, N): the same bytes
     in the reference's pack_b stream and in the native tiles (rl_weights_shard)."""
-    import ctypes
     v = [ctypes.c_int64() for _ in range(4)]
     L.call("rl_weights_shard", int(K), int(N), int(rank), int(world), *[ctypes.byref(x) for x in v])
     return tuple(x.value for x in v)
@@ -249,7 +253,6 @@ def attention(q, k, vt, nkv=None, row_limit=None, scale_log2=None, out=None, ldo
     head h at columns 128h..; bf16 rounded to bfp16 along the head dim (the out-projection's A operand), or with
     out_dtype=torch.float32 the unrounded fp32 O / l. With Hkv < H query head h reads K/V head h / (H / Hkv)
     (grouped-query attention). scale_log2 defaults to log2(e)/sqrt(128)."""
-    import math
     _check_cuda(q, k, vt, row_limit, out)
     H, Nq, _ = q.shape
     Nk = k.shape[1]
@@ -305,21 +308,24 @@ def conv2d(x_dq, w, bias, taps, out=None):
     return out
 
 
-def _check_here(*ts):
-    """CUDA tensors of the current device (any strides)."""
-    dev = None
+def _here(*ts):
+    """The current device's index, after checking that the tensors (None allowed) lie on it."""
+    dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None:
+        if t is not None and t.get_device() != dev:
             if not t.is_cuda:
                 raise ValueError("redline_tiny_b200 ops take CUDA tensors (no CPU path)")
-            if dev is None:
-                dev = torch.cuda.current_device()
-            if t.device.index != dev:
-                raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+    return dev
 
 
-def _check_int32(name, t, shape):
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+def _stream_of(dev):
+    """The current stream of device `dev` as an integer (torch.cuda.current_stream builds an object first, ~2 us)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _check_int32(name, t, *shape):
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 of shape {shape}, not {t.dtype} {tuple(t.shape)}")
 
 
@@ -332,7 +338,7 @@ class KVPool:
     value = (k - 128) * 2^(k_exp - 133); exponent 255 reads as NaN."""
 
     def __init__(self, k, v, k_exp, v_exp):
-        _check_here(k, v, k_exp, v_exp)
+        _here(k, v, k_exp, v_exp)
         if k.dim() != 5 or k.shape[4] != 128 or k.shape[3] not in (16, 32, 64, 128, 256):
             raise ValueError("cache codes must be (layers, pages, kv_heads, page, 128), page = 16, 32, 64, 128 or 256")
         exps = (*k.shape[:3], k.shape[3] // KV_BLOCK)
@@ -356,16 +362,15 @@ class KVPool:
         return (*self._ptrs[layer], self.pages, self.kv_heads, self.page)
 
 
-def _batch(pool, table, kv_len, q_start=None):
-    _check_here(pool.k, table, kv_len, q_start)
+def _batch(table, kv_len, starts, extra):
+    """Sequences and page table width of a batch's int32 arrays."""
     if table.dim() != 2 or table.shape[1] == 0:
         raise ValueError("table must be int32 (sequences, pages)")
-    B = table.shape[0]
-    _check_int32("table", table, (B, table.shape[1]))
-    _check_int32("kv_len", kv_len, (B,))
-    if q_start is not None:
-        _check_int32("q_start", q_start, (B + 1,))
-    return B
+    B, width = table.shape
+    _check_int32("table", table, B, width)
+    _check_int32("kv_len", kv_len, B)
+    _check_int32("q_start" if extra else "start", starts, B + extra)
+    return B, width
 
 
 def kv_append(pool, layer, k, v, table, kv_len, q_start):
@@ -373,37 +378,41 @@ def kv_append(pool, layer, k, v, table, kv_len, q_start):
     cache. table int32 (B, pages), kv_len int32 (B) with the new tokens counted, q_start int32 (B + 1): the new tokens
     of sequence b are rows q_start[b] .. q_start[b + 1] - 1 and take its last positions. A block's exponent grows to
     hold them, and older codes of the block are shifted. The pages written must belong to one sequence each."""
-    B = _batch(pool, table, kv_len, q_start)
-    _check_here(pool.k, k, v)
-    if k.dim() != 3 or tuple(k.shape[1:]) != (pool.kv_heads, 128) or k.shape != v.shape or k.dtype != v.dtype:
+    dev = _here(pool.k, k, v, table, kv_len, q_start)
+    B, width = _batch(table, kv_len, q_start, 1)
+    T = k.shape[0]
+    if k.shape != (T, pool.kv_heads, 128) or k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError(f"k and v must be (rows, {pool.kv_heads}, 128) of one dtype")
-    L.call("rl_kv_append", _ptr(k), *k.stride(), _ptr(v), *v.stride(), _dtype_code(k), k.shape[0], *pool._args(layer),
-           _ptr(table), table.shape[1], _ptr(kv_len), _ptr(q_start), B, _stream())
+    L.call("rl_kv_append", k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), _dtype_code(k), T, *pool._args(layer),
+           table.data_ptr(), width, kv_len.data_ptr(), q_start.data_ptr(), B, _stream_of(dev))
 
 
 def kv_read(pool, layer, table, kv_len, start, count):
     """Positions start[b] .. start[b] + count - 1 of each sequence of a layer as (k, v) bf16 (B, count, kv_heads, 128),
     exactly; zeros at and after kv_len[b]."""
-    B = _batch(pool, table, kv_len)
-    _check_here(pool.k, start)
-    _check_int32("start", start, (B,))
-    k = torch.empty((B, int(count), pool.kv_heads, 128), dtype=torch.bfloat16, device=pool.k.device)
-    v = torch.empty_like(k)
-    L.call("rl_kv_read", *pool._args(layer), _ptr(table), table.shape[1], _ptr(kv_len), _ptr(start), B, int(count),
-           _ptr(k), _ptr(v), _stream())
+    dev = _here(pool.k, table, kv_len, start)
+    B, width = _batch(table, kv_len, start, 0)
+    kv = torch.empty((2, B, count, pool.kv_heads, 128), dtype=torch.bfloat16, device=pool.k.device)
+    k, v = kv.unbind(0)
+    L.call("rl_kv_read", *pool._args(layer), table.data_ptr(), width, kv_len.data_ptr(), start.data_ptr(), B, count,
+           k.data_ptr(), v.data_ptr(), _stream_of(dev))
     return k, v
 
 
 def kv_copy_pages(pool, src, dst):
     """Copy page src[i] to page dst[i] in every layer (src, dst: sequences of ints on the host). The copies run at once:
     a page that is written is neither read nor written by another copy of the call."""
-    import array
-    _check_here(pool.k)
+    dev = _here(pool.k)
     a, b = array.array("i", src), array.array("i", dst)
     if len(a) != len(b):
         raise ValueError(f"{len(a)} source pages for {len(b)} destinations")
     L.call("rl_kv_copy_pages", *pool._ptrs[0], pool.layers, pool.pages, pool.kv_heads, pool.page, a.buffer_info()[0],
-           b.buffer_info()[0], len(a), _stream())
+           b.buffer_info()[0], len(a), _stream_of(dev))
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv_attention_workspace(dev, T, B, heads, kv_heads):
+    return max(L.lib().rl_kv_attention_workspace(T, B, heads, kv_heads), 16)
 
 
 def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_log2=None, out=None):
@@ -412,26 +421,29 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     <= kv_len[b] - n + j, or <= min(row_limit[row], kv_len[b] - 1) with row_limit int32 (T); a row that sees no key gives
     zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128). scale_log2 defaults to
     log2(e)/sqrt(128)."""
-    B = _batch(pool, table, kv_len, q_start)
-    _check_here(pool.k, q, row_limit, out)
-    if q.dim() != 3 or q.shape[2] != 128 or q.stride(2) != 1 or q.dtype != torch.bfloat16:
-        raise ValueError("q must be bf16 (rows, heads, 128) with contiguous head vectors")
-    T, H = q.shape[:2]
+    dev = _here(q, pool.k, table, kv_len, q_start, row_limit, out)
+    B, width = _batch(table, kv_len, q_start, 1)
+    if q.dim() != 3 or q.dtype is not torch.bfloat16:
+        raise ValueError("q must be bf16 (rows, heads, 128)")
+    T, H, D = q.shape
+    st, sh, sd = q.stride()
+    if D != 128 or sd != 1:
+        raise ValueError("q must be (rows, heads, 128) with contiguous head vectors")
     if row_limit is not None:
-        _check_int32("row_limit", row_limit, (T,))
+        _check_int32("row_limit", row_limit, T)
     if out is None:
         out = torch.empty((T, H * 128), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, H * 128) or (T and out.stride(1) != 1):
+    elif out.dtype is not torch.bfloat16 or out.shape != (T, H * 128) or out.stride(1) != 1:
         raise ValueError(f"out must be bf16 ({T}, {H * 128}) with contiguous rows")
-    ws = torch.empty(max(L.lib().rl_kv_attention_workspace(T, B, H, pool.kv_heads), 16), dtype=torch.uint8,
-                     device=q.device)
-    L.call("rl_kv_attention", _ptr(q), q.stride(0), q.stride(1), T, H, *pool._args(layer), _ptr(table), table.shape[1],
-           _ptr(kv_len), _ptr(q_start), B, _ptr(row_limit), _SCALE_LOG2 if scale_log2 is None else float(scale_log2),
-           _ptr(out), out.stride(0), _ptr(ws), ws.numel(), _stream())
+    ws = torch.empty(_kv_attention_workspace(dev, T, B, H, pool.kv_heads), dtype=torch.uint8, device=q.device)
+    L.call("rl_kv_attention", q.data_ptr(), st, sh, T, H, *pool._args(layer), table.data_ptr(), width,
+           kv_len.data_ptr(), q_start.data_ptr(), B, None if row_limit is None else row_limit.data_ptr(),
+           _SCALE_LOG2 if scale_log2 is None else scale_log2, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+           _stream_of(dev))
     return out
 
 
-_SCALE_LOG2 = 1.4426950408889634 / 128 ** 0.5
+_SCALE_LOG2 = math.log2(math.e) / math.sqrt(128)
 
 
 class Weight4:
@@ -441,12 +453,12 @@ class Weight4:
     def __init__(self, codes, scales, K, N, group, swiglu=False):
         self.codes, self.scales = codes, scales
         self.K, self.N, self.group, self.swiglu = int(K), int(N), int(group), bool(swiglu)
+        self._ptrs = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def from_codes(cls, codes, scales, swiglu=False):
         """codes uint8 (K, N), one value 0 .. 15 per byte, and scales bf16 (K / group, N) -> native order."""
-        import ctypes
-        _check_here(codes, scales)
+        dev = _here(codes, scales)
         _check_cuda(codes, scales)
         K, N = codes.shape
         if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or scales.shape[1] != N or \
@@ -456,7 +468,7 @@ class Weight4:
         nb = [ctypes.c_size_t(), ctypes.c_size_t()]
         L.call("rl_w4_bytes", K, N, group, int(swiglu), *[ctypes.byref(b) for b in nb])
         w, s = (torch.empty(b.value, dtype=torch.uint8, device=codes.device) for b in nb)
-        L.call("rl_w4_pack", _ptr(codes), _ptr(scales), K, N, group, int(swiglu), _ptr(w), _ptr(s), _stream())
+        L.call("rl_w4_pack", _ptr(codes), _ptr(scales), K, N, group, int(swiglu), _ptr(w), _ptr(s), _stream_of(dev))
         return cls(w, s, K, N, group, swiglu)
 
     @classmethod
@@ -468,28 +480,29 @@ class Weight4:
 def quantize_w4(B, group=64):
     """B (K, N) fp32/bf16 -> (codes uint8 (K, N), scales bf16 (K / group, N)): s = bf16(e / -8) with e the group's value
     of largest magnitude, u = clip(rint(w / s) + 8, 0, 15)."""
-    _check_here(B)
+    dev = _here(B)
     _check_cuda(B)
     K, N = B.shape
     codes = torch.empty((K, N), dtype=torch.uint8, device=B.device)
     scales = torch.empty((K // max(int(group), 1), N), dtype=torch.bfloat16, device=B.device)
-    L.call("rl_w4_quantize", _ptr(B), _dtype_code(B), K, N, int(group), _ptr(codes), _ptr(scales), _stream())
+    L.call("rl_w4_quantize", _ptr(B), _dtype_code(B), K, N, int(group), _ptr(codes), _ptr(scales), _stream_of(dev))
     return codes, scales
 
 
 def _w4(x, w, bias, epi, out, cols, out_dtype):
-    _check_here(x, w.codes, bias, out)
+    dev = _here(x, w.codes, bias, out)
     _check_cuda(x, bias, out)
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != w.K:
+    M = x.shape[0]
+    if x.shape != (M, w.K) or x.dtype is not torch.bfloat16:
         raise ValueError(f"x must be bf16 (rows, {w.K}), not {x.dtype} {tuple(x.shape)}")
-    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (w.N,)):
+    if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (w.N,)):
         raise ValueError(f"bias must be bf16 ({w.N},)")
     if out is None:
-        out = torch.empty((x.shape[0], cols), dtype=out_dtype, device=x.device)
-    elif tuple(out.shape) != (x.shape[0], cols):
-        raise ValueError(f"out must be {(x.shape[0], cols)}")
-    L.call("rl_linear_w4", _ptr(x), x.shape[0], w.K, _ptr(w.codes), _ptr(w.scales), w.N, w.group, _ptr(bias), epi,
-           _ptr(out), _dtype_code(out), _stream())
+        out = torch.empty((M, cols), dtype=out_dtype, device=x.device)
+    elif out.shape != (M, cols):
+        raise ValueError(f"out must be {(M, cols)}")
+    L.call("rl_linear_w4", x.data_ptr(), M, w.K, *w._ptrs, w.N, w.group, None if bias is None else bias.data_ptr(), epi,
+           out.data_ptr(), _dtype_code(out), _stream_of(dev))
     return out
 
 
