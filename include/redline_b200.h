@@ -393,7 +393,7 @@ int rl_set_attention_variant(int variant);
  * pool_ke / pool_ve [pages][kv_heads][page / 16] uint8; page = 16, 32, 64, 128 or 256 tokens. A block of 16 tokens of one
  * head shares one exponent: value = (u - 128) * 2^(E - 133), u = code, and E = 255 reads as NaN.
  *
- * A batch of B <= 4096 sequences lies in device memory: table (B rows of table_ld int32: the pages of the sequence in
+ * A batch of B <= 1024 sequences lies in device memory: table (B rows of table_ld int32: the pages of the sequence in
  * order), kv_len[B] (tokens in the cache, the new ones included), q_start[B + 1] (the new tokens of sequence b are rows
  * q_start[b] .. q_start[b + 1] - 1; row j of n sits at position kv_len - n + j). The kernels check what they read: a
  * sequence whose numbers are impossible is left out, a page outside the pool is skipped (its keys count as absent), and

@@ -75,7 +75,9 @@ def attention(q, k, v, limit, present=None):
     the error that half-step fp16 weights and fp32 scores leave before the output's own rounding:
     2 * 2^-11 * sum w|v| (each weight and the sum of weights off by 2^-11), the scores' fp32 sums of 128 products (128
     half steps of 2^-24 of sum |q k|, doubled for the tensor core's truncation) carried through the exponential into
-    weights and sum, and weights below fp16's normal range (absolute 2^-25 each, the largest weight being >= 1)."""
+    weights and sum, and weights below fp16's normal range: weights are kept times 2^4 and, in a block whose V exponent is
+    d <= 8 below the largest, times 2^-d, so they are off by 2^-25 2^(d - 4) there (the largest weight being >= 1) and
+    |v| <= 2^(E - d - 126) for the largest exponent E: together at most 2^-29 2^(E - 126) <= 2^-28 max |v| a key."""
     n, heads, _ = q.shape
     grp = heads // k.shape[1]
     o, bound = np.zeros(q.shape), np.zeros(q.shape)
@@ -93,7 +95,7 @@ def attention(q, k, v, limit, present=None):
             es = (np.abs(kh[keep]) @ np.abs(q[r, h])).max() / np.sqrt(128) * 128 * 2.0 ** -23
             va = np.abs(vh[keep])
             o[r, h] = w @ vh[keep]
-            bound[r, h] = (2 ** -10 + 4 * es) * (w @ va) + 2.0 ** -25 * keep.sum() * va.max(0) + 1e-30
+            bound[r, h] = (2 ** -10 + 4 * es) * (w @ va) + 2.0 ** -28 * keep.sum() * va.max() + 1e-30
     return o, bound
 
 

@@ -18,7 +18,7 @@ namespace kv {
 
 constexpr int HD = 128;     // head dim
 constexpr int BT = 16;      // tokens per block (one exponent)
-constexpr int kMaxBatch = 4096;
+constexpr int kMaxBatch = 1024;
 
 struct Pool {               // one layer
   uint8_t *k, *v, *ke, *ve;

@@ -27,9 +27,32 @@ using kv::BT;
 using kv::HD;
 
 constexpr int UNIT = 64;         // keys per unit of work
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr float kRaise = 8.0f;   // the running maximum rises only when a score exceeds it by more (log2): P <= 2^8
+constexpr float kRaise = 8.0f;   // the running maximum rises only when a score exceeds it by more (log2)
+// P is kept times 2^kUp (<= 2^12). A V block whose scale is 2^-d of the unit of O lowers its P by 2^d, which costs a
+// weight bits only below 2^(d - 18) of the largest; with d <= kWindow, below 2^-10, where they are off by 2^-21.
+constexpr int kUp = 4;
+constexpr uint32_t kWindow = 8;
+constexpr float kNone = -1e30f;  // running maximum before any key (finite: no inf - inf)
+
+// n / d for 0 <= n < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d), s = ceil(log2 d); mul d exceeds
+// 2^(31 + s) by e < d <= 2^s, so n e < 2^(31 + s) and the quotient is exact.
+struct Div {
+  uint32_t d, mul, sh;
+  static Div of(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return Div{d, static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), s};
+  }
+};
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const Div& v) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(n) * v.mul) >> 31) >> v.sh;
+}
+
+// What CTA i's task that it began and did not finish needs to be joined: its sequence's first row, the rows of a K/V
+// head, the head, the tile, and the pieces (none: 0; negative: the first lies in the CTA's second slot).
+struct Record {
+  int s0, rows, h, tile, n, pad[3];
+};
 
 struct Args {
   const uint16_t* q;
@@ -40,14 +63,10 @@ struct Args {
   float scale_log2;
   uint16_t* o;
   int64_t ldo;
-  int group;                     // query heads per K/V head
+  Div group, hkv;                // query heads per K/V head, K/V heads
+  int page_sh;                   // log2 of the page size
   float* part;                   // workspace: 2 slots per CTA of R x (128 + 2) floats
-  int4* rec;                     // workspace: per CTA, the task it began and did not finish
-};
-
-// A piece record: rows [row0, row0 + R) of task (b, h) in `n` pieces, the first in slot `slot` of this CTA.
-struct Piece {
-  int b, h, tile, n;
+  Record* rec;                   // workspace: per CTA, the task it began and did not finish
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -81,6 +100,12 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 // Bytes (u0, u1) of a word pair, as fp16 integers u - 128.
 template <int kSel>
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w) {
@@ -103,21 +128,23 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 
 // The list of units: sequence b has hkv * tiles(b) tasks of chunks(b) units each.
 __device__ __forceinline__ int64_t tiles_of(const Args& a, const kv::Seq& s, int R) {
-  return (s.n * a.group + R - 1) / R;
+  return (s.n * a.group.d + R - 1) / R;
 }
 __device__ __forceinline__ int64_t chunks_of(const kv::Seq& s) { return s.len > 0 ? (s.len + UNIT - 1) / UNIT : 1; }
 
 // Prefix sums of the sequences' units into `pre` (B + 1 values), by the whole CTA.
-__device__ __forceinline__ void unit_prefix(const Args& a, int R, int64_t* pre, int64_t* warp_sum) {
+template <int kWarps>
+__device__ __forceinline__ void unit_prefix(const Args& a, int R, int64_t* pre, int64_t* warp_sum, int4* seqs) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) pre[0] = 0;
   int64_t base = 0;
-  for (int b0 = 0; b0 < a.batch.B; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.batch.B; b0 += 32 * kWarps) {
     const int b = b0 + threadIdx.x;
     int64_t u = 0;
     if (b < a.batch.B) {
       const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
-      if (s.ok) u = tiles_of(a, s, R) * chunks_of(s) * a.pool.hkv;
+      seqs[b] = make_int4(static_cast<int>(s.s0), static_cast<int>(s.n), static_cast<int>(s.len), 0);
+      if (s.ok) u = tiles_of(a, s, R) * chunks_of(s) * a.hkv.d;
       else if (blockIdx.x == 0) report(kErrBadArgument);
     }
 #pragma unroll
@@ -139,16 +166,48 @@ template <int NT>
 struct Acc {
   float o[NT][8][4];     // O^T: dims 16g + 2i (+1 for [2], [3]), rows 2c, 2c + 1 of n-tile nt
   float m[NT][2], l[NT][2];
+  int er;                // O is in units of 2^(er - 133)
 };
+
+// P^T of a block times 2^shift, in the B layout; the row sums add the rounded weights times `unit`.
+template <int NT>
+__device__ __forceinline__ void weights(const float (&s)[NT][4], Acc<NT>& acc, float shift, float unit, uint32_t (&p)[NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float m0 = acc.m[nt][0] - shift, m1 = acc.m[nt][1] - shift;
+    const uint32_t lo = pack_h2(exp2_approx(s[nt][0] - m0), exp2_approx(s[nt][1] - m1));
+    const uint32_t hi = pack_h2(exp2_approx(s[nt][2] - m0), exp2_approx(s[nt][3] - m1));
+    const float2 f = unpack_h2(lo), h = unpack_h2(hi);
+    acc.l[nt][0] = fmaf(unit, f.x + h.x, acc.l[nt][0]);
+    acc.l[nt][1] = fmaf(unit, f.y + h.y, acc.l[nt][1]);
+    p[nt][0] = movmatrix(lo);
+    p[nt][1] = movmatrix(hi);
+  }
+}
+
+// The eight V^T fragments of a block (dims 16g + 2i, + 1), each handed to `f` for every n-tile.
+template <int NT, typename F>
+__device__ __forceinline__ void add_values(const uint4 (&vr)[4], F f) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t t0 = (&vr[0].x)[w], t1 = (&vr[1].x)[w], t2 = (&vr[2].x)[w], t3 = (&vr[3].x)[w];
+#pragma unroll
+    for (int hl = 0; hl < 2; ++hl) {
+      const uint32_t x = __byte_perm(t0, t1, hl ? 0x7362 : 0x5140), y = __byte_perm(t2, t3, hl ? 0x7362 : 0x5140);
+      const uint32_t a0 = codes_h2<0x4140>(x), a1 = codes_h2<0x4342>(x);
+      const uint32_t a2 = codes_h2<0x4140>(y), a3 = codes_h2<0x4342>(y);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) f(2 * w + hl, a0, a1, a2, a3, nt);
+    }
+  }
+}
 
 // One warp, one block of 16 keys starting at position pos0.
 template <int NT>
 __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&vr)[4], uint32_t ke, uint32_t ve,
-                                           int64_t pos0, const uint32_t (&qf)[16], uint32_t q_at, const float (&qs)[NT][2],
+                                           int pos0, const uint32_t (&qf)[16], uint32_t q_at, const float (&qs)[NT][2],
                                            const int (&lim)[NT][2], int lim_min, int g, Acc<NT>& acc) {
   float s[NT][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
   const uint32_t* k0[2] = {&kr[0].x, &kr[1].x};   // token g: dims 16c.., 64 + 16c..
   const uint32_t* k1[2] = {&kr[2].x, &kr[3].x};   // token g + 8
 #pragma unroll
@@ -165,24 +224,35 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
     for (int nt = 0; nt < NT; ++nt) {
       uint4 q = make_uint4(qf[4 * jj], qf[4 * jj + 1], qf[4 * jj + 2], qf[4 * jj + 3]);
       if (NT > 1) q = lds128(q_at + (nt * 4 + jj) * 512);
-      mma(s[nt], A[0][0], A[0][1], A[0][2], A[0][3], q.x, q.y);
+      if (jj == 0) mma_zero(s[nt], A[0][0], A[0][1], A[0][2], A[0][3], q.x, q.y);
+      else mma(s[nt], A[0][0], A[0][1], A[0][2], A[0][3], q.x, q.y);
       mma(s[nt], A[1][0], A[1][1], A[1][2], A[1][3], q.z, q.w);
     }
   }
   const float ks = ke == 255u ? __uint_as_float(0x7FC00000u) : bfp16_scale(ke);
-  bool raise = false;
+  // units of O: V blocks bring their scale in through P while it is within 2^kWindow of the unit
+  const int ev = ve == 255u ? acc.er : static_cast<int>(ve);
+  int d = acc.er - ev;
+  uint32_t p[NT][2];
+  bool change = static_cast<uint32_t>(d) > kWindow;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[nt][i] = s[nt][i] * ks * qs[nt][i & 1];
+    const float f0 = ks * qs[nt][0], f1 = ks * qs[nt][1];
+    s[nt][0] *= f0, s[nt][1] *= f1, s[nt][2] *= f0, s[nt][3] *= f1;
     if (pos0 + BT - 1 > lim_min) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (pos0 + g + 8 * (i >> 1) > lim[nt][i & 1]) s[nt][i] = -INFINITY;
     }
-    raise |= fmaxf(s[nt][0], s[nt][2]) > acc.m[nt][0] + kRaise || fmaxf(s[nt][1], s[nt][3]) > acc.m[nt][1] + kRaise;
+    change |= fmaxf(s[nt][0], s[nt][2]) > acc.m[nt][0] + kRaise || fmaxf(s[nt][1], s[nt][3]) > acc.m[nt][1] + kRaise;
   }
-  if (__any_sync(0xffffffffu, raise)) {
+  if (__any_sync(0xffffffffu, change)) {
+    float to = 1.0f;
+    if (ev > acc.er) {
+      to = exp2f(static_cast<float>(acc.er - ev));
+      acc.er = ev;
+    }
+    d = acc.er - ev;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -195,55 +265,38 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
         const float alpha = m == acc.m[nt][c] ? 1.0f : exp2_approx(acc.m[nt][c] - m);
         acc.m[nt][c] = m;
         acc.l[nt][c] *= alpha;
+        const float f = alpha * to;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          acc.o[nt][i][c] *= alpha;
-          acc.o[nt][i][c + 2] *= alpha;
+          acc.o[nt][i][c] *= f;
+          acc.o[nt][i][c + 2] *= f;
         }
       }
-  }
-  uint32_t p[NT][2];
+    if (d > static_cast<int>(kWindow)) {
+      // a block far below the unit (zeros, for one): its product is scaled as it is added, and the code below adds none
+      const float vs = exp2f(static_cast<float>(-d));
+      weights<NT>(s, acc, static_cast<float>(kUp), 1.0f, p);
+      add_values<NT>(vr, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int nt) {
+        float t[4];
+        mma_zero(t, a0, a1, a2, a3, p[nt][0], p[nt][1]);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float m0 = acc.m[nt][0] == -INFINITY ? 0.0f : acc.m[nt][0];
-    const float m1 = acc.m[nt][1] == -INFINITY ? 0.0f : acc.m[nt][1];
-    const uint32_t lo = pack_h2(exp2_approx(s[nt][0] - m0), exp2_approx(s[nt][1] - m1));
-    const uint32_t hi = pack_h2(exp2_approx(s[nt][2] - m0), exp2_approx(s[nt][3] - m1));
-    const float2 f = unpack_h2(lo), h = unpack_h2(hi);
-    acc.l[nt][0] += f.x + h.x;
-    acc.l[nt][1] += f.y + h.y;
-    p[nt][0] = movmatrix(lo);
-    p[nt][1] = movmatrix(hi);
+        for (int j = 0; j < 4; ++j) acc.o[nt][i][j] = fmaf(vs, t[j], acc.o[nt][i][j]);
+      });
+      d = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = -INFINITY;
+    }
   }
-  if (ve == 255u) {   // a block with a NaN or an infinity: NaN for the rows that see it, nothing for the others
-    const float nan = __uint_as_float(0x7FC00000u);
+  weights<NT>(s, acc, static_cast<float>(kUp - d), __uint_as_float(static_cast<uint32_t>(127 + d) << 23), p);
+  add_values<NT>(vr, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int nt) {
+    mma(acc.o[nt][i], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+  });
+  if (ve == 255u) {   // a block with a NaN or an infinity: NaN for the rows that see it (the codes are small integers)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        if (pos0 <= lim[nt][c]) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc.o[nt][i][c] = acc.o[nt][i][c + 2] = nan;
-        }
-    return;
-  }
-  const float vs = bfp16_scale(ve);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const uint32_t t0 = (&vr[0].x)[w], t1 = (&vr[1].x)[w], t2 = (&vr[2].x)[w], t3 = (&vr[3].x)[w];
-#pragma unroll
-    for (int hl = 0; hl < 2; ++hl) {
-      const uint32_t x = __byte_perm(t0, t1, hl ? 0x7362 : 0x5140), y = __byte_perm(t2, t3, hl ? 0x7362 : 0x5140);
-      const uint32_t a0 = codes_h2<0x4140>(x), a1 = codes_h2<0x4342>(x);
-      const uint32_t a2 = codes_h2<0x4140>(y), a3 = codes_h2<0x4342>(y);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        mma(t, a0, a1, a2, a3, p[nt][0], p[nt][1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc.o[nt][2 * w + hl][i] = fmaf(vs, t[i], acc.o[nt][2 * w + hl][i]);
-      }
-    }
+        if (pos0 <= lim[nt][c]) acc.l[nt][c] = __uint_as_float(0x7FC00000u);
   }
 }
 
@@ -252,29 +305,35 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
 template <int NT>
 struct Cfg {
   static constexpr int R = 8 * NT;
-  static constexpr int kStages = NT == 4 ? 4 : 3;
+  // NT = 1: 4 CTAs of 4 warps hide each other's starts and ends of tasks. Medians on one box, 64 sequences of up to 8192
+  // tokens (564 MB) / one of 131071 (269 MB): 4 x 4 warps 102 / 55 us, 2 x 8 116 / 51, 1 x 16 144 / 57; 2 stages instead
+  // of 3 the same.
+  static constexpr int kWarps = 4;
   static constexpr int kCtas = NT == 1 ? 4 : 2;                       // resident per SM
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kStages = NT == 1 ? 3 : 5;
   static constexpr int kRing = kWarps * kStages * 2 * BT * HD;
   static constexpr int kOut = kWarps * R * HD * 4;
   static constexpr int kBody = kRing > kOut ? kRing : kOut;
   static constexpr int kQ = NT == 1 ? 0 : NT * 16 * 32 * 4;            // q fragments, where registers cannot hold them
-  static size_t smem(int B) { return kBody + kQ + kWarps * R * 8 + (kWarps + B + 1) * sizeof(int64_t); }
+  static size_t smem(int B) { return kBody + kQ + kWarps * R * 8 + B * 16 + (kWarps + B + 1) * 8; }
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const Args a) {
-  constexpr int R = 8 * NT;
+__global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kernel(const Args a) {
+  constexpr int R = 8 * NT, kWarps = Cfg<NT>::kWarps;
   constexpr int S = Cfg<NT>::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   float* so = reinterpret_cast<float*>(smem);                        // [warp][row][128]
   uint8_t* sq = smem + Cfg<NT>::kBody;                               // [n-tile][4][lane] x 16 bytes
   float* sm = reinterpret_cast<float*>(sq + Cfg<NT>::kQ);            // [warp][row] maxima
   float* sl = sm + kWarps * R;                                       // [warp][row] sums
-  int64_t* warp_sum = reinterpret_cast<int64_t*>(sl + kWarps * R);
+  int4* seqs = reinterpret_cast<int4*>(sl + kWarps * R);              // first row, rows and length of each sequence
+  int64_t* warp_sum = reinterpret_cast<int64_t*>(seqs + a.batch.B);
   int64_t* pre = warp_sum + kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  unit_prefix(a, R, pre, warp_sum);
+  unit_prefix<kWarps>(a, R, pre, warp_sum, seqs);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t U = pre[a.batch.B];
   const int64_t C = min(static_cast<int64_t>(gridDim.x), U);        // every working CTA has at least one unit
@@ -282,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
   const int64_t u_end = idle ? 0 : (blockIdx.x + 1) * U / C;
   int64_t u = idle ? 0 : blockIdx.x * U / C;
   bool first = true;
-  Piece rec{0, 0, 0, 0};
+  Record rec = {};
   int b = 0;
 
   // ring addresses of this lane. Row r of a block keeps its 16-byte chunk j at chunk j ^ f(r), f = 4 (r & 1) for K and
@@ -300,13 +359,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
       if (pre[mid] <= u) lo = mid; else hi = mid;
     }
     b = lo;
-    const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
-    const int64_t nch = chunks_of(s);
-    const int64_t task = (u - pre[b]) / nch, ch0 = (u - pre[b]) - task * nch;
+    const int4 sq4 = seqs[b];
+    const kv::Seq s{sq4.x, sq4.y, sq4.z, true};
+    const int64_t nch = chunks_of(s), off = u - pre[b];
+    const uint32_t task = static_cast<uint32_t>(off < (1ll << 31) ? static_cast<uint32_t>(off) / static_cast<uint32_t>(nch)
+                                                                  : off / nch);
+    const int64_t ch0 = off - task * nch;
     const int64_t ch1 = min(nch, ch0 + (u_end - u));
-    const int h = static_cast<int>(task % a.pool.hkv);
-    const int64_t tile = task / a.pool.hkv;
-    const int64_t rows = s.n * a.group;                              // rows of this K/V head
+    const uint32_t tile = task / a.hkv;
+    const int h = static_cast<int>(task - tile * a.hkv.d);
+    const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;    // rows of this K/V head
+    const uint32_t row0 = tile * R;
 
     uint32_t qf[16];
     float qs[NT][2];
@@ -316,11 +379,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int64_t rr = tile * R + nt * 8 + 2 * c + k;
+        const uint32_t rr = row0 + nt * 8 + 2 * c + k;
         int64_t L = -1;
         if (rr < rows) {
-          L = s.len - s.n + rr / a.group;
-          if (a.row_limit) L = min(s.len - 1, static_cast<int64_t>(__ldg(a.row_limit + s.s0 + rr / a.group)));
+          const uint32_t j = rr / a.group;
+          L = s.len - s.n + j;
+          if (a.row_limit) L = min(s.len - 1, static_cast<int64_t>(__ldg(a.row_limit + s.s0 + j)));
         }
         lim[nt][k] = static_cast<int>(max(L, static_cast<int64_t>(-1)));
         lim_max = max(lim_max, lim[nt][k]);
@@ -332,50 +396,55 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
 
-    // the warp's blocks: every fourth of the run. Lane j holds the pool index of block 32 t + j, one chunk ahead.
+    // the warp's blocks: every kWarps-th of the run. Lane j holds the pool index of block 32 t + j, one chunk ahead.
     const int64_t key_end = min(ch1 * UNIT, static_cast<int64_t>(lim_max) + 1);
     const int64_t pos0 = ch0 * UNIT + warp * BT;
-    const int n = key_end > pos0 ? static_cast<int>((key_end - pos0 + UNIT - 1) / UNIT) : 0;
+    const int n = key_end > pos0 ? static_cast<int>((key_end - pos0 + kWarps * BT - 1) / (kWarps * BT)) : 0;
     auto block_of = [&](int k) -> int {
       if (k >= n) return -1;
-      const int64_t blk = kv::block_index(a.pool, a.batch, b, pos0 + static_cast<int64_t>(k) * UNIT, h);
-      if (blk < 0) report(kErrBadArgument);                          // a page outside the pool: its keys are absent
-      return static_cast<int>(blk);
+      const uint32_t pos = static_cast<uint32_t>(pos0) + k * (kWarps * BT);
+      const int pg = __ldg(a.batch.table + b * a.batch.ld + (pos >> a.page_sh));
+      if (static_cast<uint32_t>(pg) >= a.pool.pages) {               // a page outside the pool: its keys are absent
+        report(kErrBadArgument);
+        return -1;
+      }
+      return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + ((pos & (a.pool.page - 1)) >> 4);
     };
     int idx = block_of(lane), idx_next = block_of(32 + lane);
-    uint32_t ex[S];                                                  // ke | ve << 8 | present << 16 of the ring's blocks
-    auto issue = [&](int k, uint32_t& e) {
+    uint32_t ke[S], ve[S];                                           // of the ring's blocks
+    int at_pos[S];                                                   // first position, or beyond every limit
+    auto issue = [&](int k, int j) {
       if (k < n) {
         if ((k & 31) == 0 && k > 0) {
           idx = idx_next;
           idx_next = block_of(k + 32 + lane);
         }
-        const int64_t blk = __shfl_sync(0xffffffffu, idx, k & 31);
-        e = 0;
-        if (blk >= 0) {
-          e = a.pool.ke[blk] | (a.pool.ve[blk] << 8) | 0x10000u;
-          const uint8_t* kp = a.pool.k + blk * (BT * HD) + lane * 16;
-          const uint8_t* vp = a.pool.v + blk * (BT * HD) + lane * 16;
-          const uint32_t d = ring + (k % S) * (2 * BT * HD) + wr * HD;
+        const int found = __shfl_sync(0xffffffffu, idx, k & 31);
+        const int64_t blk = max(found, 0);                           // an absent block reads as block 0, fully masked
+        at_pos[j] = found < 0 ? 0x7FFFFF00 : static_cast<int>(pos0) + k * (kWarps * BT);
+        ke[j] = a.pool.ke[blk], ve[j] = a.pool.ve[blk];
+        const uint8_t* kp = a.pool.k + blk * (BT * HD) + lane * 16;
+        const uint8_t* vp = a.pool.v + blk * (BT * HD) + lane * 16;
+        const uint32_t d = ring + j * (2 * BT * HD) + wr * HD;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) cp_async16(d + j * 4 * HD + ((wc ^ ((wr & 1) * 4)) << 4), kp + j * 512);
+        for (int i = 0; i < 4; ++i) cp_async16(d + i * 4 * HD + ((wc ^ ((wr & 1) * 4)) << 4), kp + i * 512);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            cp_async16(d + BT * HD + j * 4 * HD + ((wc ^ ((((wr + 4 * j) >> 1) & 3) * 2)) << 4), vp + j * 512);
-        }
+        for (int i = 0; i < 4; ++i)
+          cp_async16(d + BT * HD + i * 4 * HD + ((wc ^ ((((wr + 4 * i) >> 1) & 3) * 2)) << 4), vp + i * 512);
       }
       cp_commit();
     };
 #pragma unroll
-    for (int k = 0; k < S - 1; ++k) issue(k, ex[k]);
+    for (int k = 0; k < S - 1; ++k) issue(k, k);
 
     // q of the tile, while the first blocks are on their way
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int64_t r = tile * R + nt * 8 + g;                       // the row whose q this lane loads
+      const uint32_t r = row0 + nt * 8 + g;                          // the row whose q this lane loads
       uint4 w[4] = {};
       if (r < rows) {
-        const uint16_t* p = a.q + (s.s0 + r / a.group) * a.q_st + (h * a.group + r % a.group) * a.q_sh + 16 * c;
+        const uint32_t j = r / a.group;
+        const uint16_t* p = a.q + (s.s0 + j) * a.q_st + (h * a.group.d + r - j * a.group.d) * a.q_sh + 16 * c;
         w[0] = *reinterpret_cast<const uint4*>(p), w[1] = *reinterpret_cast<const uint4*>(p + 8);
         w[2] = *reinterpret_cast<const uint4*>(p + 64), w[3] = *reinterpret_cast<const uint4*>(p + 72);
       }
@@ -408,9 +477,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
     const uint32_t q_at = smem_u32(sq) + lane * 16;
 
     Acc<NT> acc;
+    acc.er = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      acc.m[nt][0] = acc.m[nt][1] = -INFINITY;
+      acc.m[nt][0] = acc.m[nt][1] = kNone;
       acc.l[nt][0] = acc.l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc.o[nt][i][0] = acc.o[nt][i][1] = acc.o[nt][i][2] = acc.o[nt][i][3] = 0.0f;
@@ -422,23 +492,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
         if (i < n) {
           cp_wait<S - 2>();
           __syncwarp();        // block i of every lane is in; every lane is done with block i - 1
-          issue(i + S - 1, ex[(j + S - 1) % S]);
-          if (ex[j] & 0x10000u) {
-            const uint32_t at = ring + j * (2 * BT * HD);
-            uint4 kr[4], vr[4];
-            kr[0] = lds128(at + k_ld), kr[1] = lds128(at + (k_ld ^ 64));
-            kr[2] = lds128(at + k_ld + 8 * HD), kr[3] = lds128(at + (k_ld ^ 64) + 8 * HD);
-            vr[0] = lds128(at + v_ld), vr[1] = lds128(at + v_ld + HD);
-            vr[2] = lds128(at + v_ld + 8 * HD), vr[3] = lds128(at + v_ld + 9 * HD);
-            block_step<NT>(kr, vr, ex[j] & 255u, ex[j] >> 8 & 255u, pos0 + static_cast<int64_t>(i) * UNIT, qf, q_at, qs, lim,
-                           lim_min, g, acc);
-          }
+          issue(i + S - 1, (j + S - 1) % S);
+          const uint32_t at = ring + j * (2 * BT * HD);
+          uint4 kr[4], vr[4];
+          kr[0] = lds128(at + k_ld), kr[1] = lds128(at + (k_ld ^ 64));
+          kr[2] = lds128(at + k_ld + 8 * HD), kr[3] = lds128(at + (k_ld ^ 64) + 8 * HD);
+          vr[0] = lds128(at + v_ld), vr[1] = lds128(at + v_ld + HD);
+          vr[2] = lds128(at + v_ld + 8 * HD), vr[3] = lds128(at + v_ld + 9 * HD);
+          block_step<NT>(kr, vr, ke[j], ve[j], at_pos[j], qf, q_at, qs, lim, lim_min, g, acc);
         }
       }
     }
     cp_wait<0>();
     __syncthreads();           // every warp is done with the ring
 
+    const float ou = bfp16_scale(static_cast<uint32_t>(acc.er));
     // join the warps: (O, m, l) of each through shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -453,30 +521,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
         float* d = so + (warp * R + row) * HD + 16 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          reinterpret_cast<float4*>(d)[i] = make_float4(acc.o[nt][2 * i][k], acc.o[nt][2 * i][k + 2],
-                                                        acc.o[nt][2 * i + 1][k], acc.o[nt][2 * i + 1][k + 2]);
+          reinterpret_cast<float4*>(d)[i] = make_float4(acc.o[nt][2 * i][k] * ou, acc.o[nt][2 * i][k + 2] * ou,
+                                                        acc.o[nt][2 * i + 1][k] * ou, acc.o[nt][2 * i + 1][k + 2] * ou);
       }
     __syncthreads();
     const bool whole = ch0 == 0 && ch1 == nch;
     float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * R * (HD + 2);
-    const int d = threadIdx.x;
-    for (int row = 0; row < R; ++row) {
-      const int64_t r = tile * R + row;
+    const int d = threadIdx.x % HD;
+    for (int row = threadIdx.x / HD; row < R; row += kWarps * 32 / HD) {
+      const uint32_t r = row0 + row, j = r / a.group;
       if (r >= rows) break;
       float m = sm[row];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sm[w * R + row]);
-      const float mz = m == -INFINITY ? 0.0f : m;
       float l = 0.0f, o = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(sm[w * R + row] - mz);
+        const float f = exp2_approx(sm[w * R + row] - m);
         l += f * sl[w * R + row];
         o += f * so[(w * R + row) * HD + d];
       }
       if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        a.o[(s.s0 + r / a.group) * a.ldo + (h * a.group + r % a.group) * HD + d] =
+        a.o[(s.s0 + j) * a.ldo + (h * a.group.d + r - j * a.group.d) * HD + d] =
             __bfloat16_as_ushort(__float2bfloat16_rn(o * inv));
       } else {
         part[row * HD + d] = o;
@@ -486,56 +553,93 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) attend_kernel(const 
     if (!whole && ch0 == 0) {
       // the pieces end in the CTA that holds the task's last unit x: floor(j U / C) <= x < floor((j + 1) U / C)
       const int64_t x = u + nch - 1;
-      rec = Piece{b, h, static_cast<int>(tile), static_cast<int>(((x + 1) * C - 1) / U - blockIdx.x) + 1};
-      if (!first) rec.n = -rec.n;                                    // the first piece lies in the CTA's second slot
+      const int pieces = static_cast<int>(((x + 1) * C - 1) / U - blockIdx.x) + 1;
+      rec = Record{static_cast<int>(s.s0), static_cast<int>(rows), h, static_cast<int>(tile), first ? pieces : -pieces, {}};
     }
     u += ch1 - ch0;
     first = false;
     __syncthreads();
   }
-  if (threadIdx.x == 0) a.rec[blockIdx.x] = make_int4(rec.b, rec.h, rec.tile, rec.n);
+  if (threadIdx.x == 0) a.rec[blockIdx.x] = rec;
 }
 
-// CTA i joins the pieces of the task that CTA i of attend_kernel began and did not finish: a warp per row, 4 dims a lane.
-// Launched while attend_kernel still runs (its CTAs need no more than a slot), it waits for that grid's end.
-constexpr int kJoin = 8;   // warps
+// CTA i joins the pieces of the task that CTA i of attend_kernel began and did not finish: kJoin / 8 warps to a row, each
+// a share of the pieces with a running maximum (all loads independent of it), then the shares in order. Launched while
+// attend_kernel still runs, it waits for that grid's end.
+constexpr int kJoin = 16;   // warps
 template <int NT>
 __global__ void __launch_bounds__(32 * kJoin) combine_kernel(const Args a) {
   constexpr int R = 8 * NT;
   constexpr int64_t kSlot = R * (HD + 2);
-  const int lane = threadIdx.x & 31;
+  constexpr int kShares = kJoin / 8;
+  __shared__ float4 so[kShares][8][32];
+  __shared__ float2 sml[kShares][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 rec = a.rec[blockIdx.x];
-  if (rec.w == 0) return;
-  const int pieces = abs(rec.w);
-  const kv::Seq s = kv::load_seq(a.batch, rec.x, a.pool.page);
-  const int64_t rows = s.n * a.group;
+  const Record rec = a.rec[blockIdx.x];
+  if (rec.n == 0) return;
+  const int pieces = abs(rec.n);
   // piece 0 may lie in the CTA's second slot; the others in the first slots of the CTAs behind
   const float* base = a.part + static_cast<int64_t>(blockIdx.x) * 2 * kSlot;
-  auto piece = [&](int j) { return base + (j == 0 ? (rec.w < 0 ? kSlot : 0) : j * 2 * kSlot); };
-  for (int row = threadIdx.x >> 5; row < R; row += kJoin) {
-    const int64_t r = static_cast<int64_t>(rec.z) * R + row;
-    if (r >= rows) break;
-    float m = -INFINITY;
-    for (int j = lane; j < pieces; j += 32) m = fmaxf(m, piece(j)[R * HD + row]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float z = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
+  const int share = warp >> 3;
+  for (int row0 = 0; row0 < R; row0 += 8) {
+    const int row = row0 + (warp & 7);
+    const uint32_t r = static_cast<uint32_t>(rec.tile) * R + row;
+    float m = kNone, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int j = 0; j < pieces; ++j) {
-      const float* p = piece(j);
-      const float4 v = *reinterpret_cast<const float4*>(p + row * HD + 4 * lane);
-      const float f = exp2f(p[R * HD + row] - z);
-      l = fmaf(f, p[R * HD + R + row], l);
-      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* d = a.o + (s.s0 + r / a.group) * a.ldo + (rec.y * a.group + r % a.group) * HD + 4 * lane;
-    const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    if (r < static_cast<uint32_t>(rec.rows)) {
+      for (int j0 = share; j0 < pieces; j0 += 8 * kShares) {
+        float4 v[8];
+        float mj[8], lj[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+        for (int i = 0; i < 8; ++i) {       // eight pieces on their way at once
+          const int j = j0 + i * kShares;
+          v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mj[i] = kNone, lj[i] = 0.0f;
+          if (j < pieces) {
+            const float* p = base + (j == 0 ? (rec.n < 0 ? kSlot : 0) : j * 2 * kSlot);
+            v[i] = __ldcg(reinterpret_cast<const float4*>(p + row * HD) + lane);
+            mj[i] = __ldcg(p + R * HD + row), lj[i] = __ldcg(p + R * HD + R + row);
+          }
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, mj[i]);
+        const float fa = exp2_approx(m - mn);
+        m = mn;
+        l *= fa, o.x *= fa, o.y *= fa, o.z *= fa, o.w *= fa;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = exp2_approx(mj[i] - mn);
+          l = fmaf(f, lj[i], l);
+          o.x = fmaf(f, v[i].x, o.x), o.y = fmaf(f, v[i].y, o.y), o.z = fmaf(f, v[i].z, o.z), o.w = fmaf(f, v[i].w, o.w);
+        }
+      }
+    }
+    if (share > 0) {
+      so[share][warp & 7][lane] = o;
+      if (lane == 0) sml[share][warp & 7] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (share == 0 && r < static_cast<uint32_t>(rec.rows)) {
+#pragma unroll
+      for (int j = 1; j < kShares; ++j) {
+        const float4 v = so[j][warp][lane];
+        const float2 ml = sml[j][warp];
+        const float mn = fmaxf(m, ml.x);
+        const float fa = exp2_approx(m - mn), fb = exp2_approx(ml.x - mn);
+        m = mn;
+        l = fmaf(fb, ml.y, l * fa);
+        o.x = fmaf(fb, v.x, o.x * fa), o.y = fmaf(fb, v.y, o.y * fa);
+        o.z = fmaf(fb, v.z, o.z * fa), o.w = fmaf(fb, v.w, o.w * fa);
+      }
+      const uint32_t jr = r / a.group;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint16_t* d = a.o + (rec.s0 + jr) * a.ldo + (rec.h * a.group.d + r - jr * a.group.d) * HD + 4 * lane;
+      const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+    }
+    __syncthreads();
   }
 }
 
@@ -554,7 +658,7 @@ inline int launch(const Args& a, cudaStream_t st) {
   const int ctas = ctas_of(NT);
   RL_TRY_CUDA(cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch))));
-  attend_kernel<NT><<<ctas, kThreads, smem, st>>>(a);
+  attend_kernel<NT><<<ctas, Cfg<NT>::kThreads, smem, st>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
@@ -578,7 +682,7 @@ size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads) {
   using namespace rl;
   if (T <= 0 || B <= 0 || kv_heads <= 0 || heads <= 0) return 0;
   const int nt = kvattn::tile_n(T, B, heads / kv_heads);
-  return kvattn::part_bytes(nt) + static_cast<size_t>(kvattn::ctas_of(nt)) * sizeof(int4);
+  return kvattn::part_bytes(nt) + static_cast<size_t>(kvattn::ctas_of(nt)) * sizeof(kvattn::Record);
 }
 
 int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, int heads, const uint8_t* pool_k,
@@ -599,6 +703,7 @@ int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, in
              heads, kv_heads);
   RL_REQUIRE(pages * kv_heads * (page / kv::BT) <= INT32_MAX, RL_ERR_ARGUMENT, "rl_kv_attention: %lld pages",
              (long long)pages);
+  RL_REQUIRE(T * heads < (1ll << 31), RL_ERR_ARGUMENT, "rl_kv_attention: %lld rows of %d heads", (long long)T, heads);
   RL_REQUIRE(table_ld * page <= (1 << 30), RL_ERR_ARGUMENT, "rl_kv_attention: sequences of up to %lld tokens",
              (long long)(table_ld * page));
   if (T == 0 || B == 0) return RL_OK;
@@ -613,10 +718,12 @@ int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, in
   RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_attention: needs an sm_100 device");
   a.q = q, a.q_st = q_st, a.q_sh = q_sh;
   a.row_limit = row_limit, a.scale_log2 = scale_log2;
-  a.o = o, a.ldo = ldo, a.group = heads / kv_heads;
-  const int nt = kvattn::tile_n(T, B, a.group);
+  a.o = o, a.ldo = ldo;
+  a.group = kvattn::Div::of(heads / kv_heads), a.hkv = kvattn::Div::of(kv_heads);
+  a.page_sh = __builtin_ctz(page);
+  const int nt = kvattn::tile_n(T, B, heads / kv_heads);
   a.part = static_cast<float*>(workspace);
-  a.rec = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + kvattn::part_bytes(nt));
+  a.rec = reinterpret_cast<kvattn::Record*>(static_cast<uint8_t*>(workspace) + kvattn::part_bytes(nt));
   switch (nt) {
     case 1: return kvattn::launch<1>(a, stream);
     case 2: return kvattn::launch<2>(a, stream);

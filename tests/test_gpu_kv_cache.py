@@ -217,6 +217,24 @@ def test_attention_sharp_and_wide_scores(env):
     check_attention(got, *c.oracle(q))
 
 
+def test_attention_blocks_of_very_different_scale(env):
+    """V and K blocks from 2^-40 to 2^40 and all-zero ones, in every order."""
+    torch, ops, L, dev = env
+    c = Case(torch, ops, dev, [700, 300], [1, 3], 2, 16, seed=15)
+    for cache, exps in ((c.k, c.pool.k_exp), (c.v, c.pool.v_exp)):
+        e = c.rng.choice([0, 90, 120, 125, 127, 128, 130, 138, 160], cache.exps.shape).astype(np.uint8)
+        if cache is c.k:
+            e = np.minimum(e, 130)
+        cache.exps[:] = e
+        exps[0] = torch.from_numpy(e).to(dev)
+    c.v.codes[c.v.exps.repeat(16, 2) == 0] = 128
+    c.pool.v[0] = torch.from_numpy(c.v.codes).to(dev)
+    q = O.bf16_round(c.rng.standard_normal((c.T, 4, 128)).astype(np.float32))
+    got = ops.kv_attention(bf16(torch, q, dev), *c.args())
+    ops.device_status()
+    check_attention(got, *c.oracle(q))
+
+
 def test_attention_row_limits(env):
     """Per-row limits: none visible (zeros), one key, past the end, and beyond the causal limit."""
     torch, ops, L, dev = env

@@ -35,7 +35,7 @@ def append_args(**k):
 @pytest.mark.parametrize("change,status,text", [
     (dict(pool=None), -1, b"NULL pool"), (dict(page=48), -1, b"page size"), (dict(pages=0), -1, b"pages"),
     (dict(hkv=0), -1, b"kv_heads"), (dict(pool=P + 1), -2, b"aligned"), (dict(table=None), -1, b"table"),
-    (dict(B=4097), -1, b"sequences"), (dict(ld=0), -1, b"table"), (dict(T=-1), -1, b"rows"), (dict(dtype=7), -1, b"dtype"),
+    (dict(B=1025), -1, b"sequences"), (dict(ld=0), -1, b"table"), (dict(T=-1), -1, b"rows"), (dict(dtype=7), -1, b"dtype"),
     (dict(k=None), -1, b"NULL"), (dict(k=P + 1), -2, b"aligned"), (dict(table=P + 2), -2, b"int32"),
 ])
 def test_append(lib, change, status, text):
