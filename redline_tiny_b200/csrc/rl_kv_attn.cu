@@ -120,11 +120,8 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
+// (a plain load, which the compiler may place among the matrix instructions)
+__device__ __forceinline__ uint4 lds128(const uint8_t* a) { return *reinterpret_cast<const uint4*>(a); }
 
 // The list of units: sequence b has hkv * tiles(b) tasks of chunks(b) units each.
 __device__ __forceinline__ int64_t tiles_of(const Args& a, const kv::Seq& s, int R) {
@@ -205,7 +202,7 @@ __device__ __forceinline__ void add_values(const uint4 (&vr)[4], F f) {
 // One warp, one block of 16 keys starting at position pos0.
 template <int NT>
 __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&vr)[4], uint32_t ke, uint32_t ve,
-                                           int pos0, const uint32_t (&qf)[16], uint32_t q_at, const float (&qs)[NT][2],
+                                           int pos0, const uint32_t (&qf)[16], const uint8_t* q_at, const float (&qs)[NT][2],
                                            const int (&lim)[NT][2], int lim_min, int g, Acc<NT>& acc) {
   float s[NT][4];
   const uint32_t* k0[2] = {&kr[0].x, &kr[1].x};   // token g: dims 16c.., 64 + 16c..
@@ -474,7 +471,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     }
 
     if (NT > 1) __syncthreads();
-    const uint32_t q_at = smem_u32(sq) + lane * 16;
+    const uint8_t* q_at = sq + lane * 16;
 
     Acc<NT> acc;
     acc.er = 0;
@@ -493,7 +490,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
           cp_wait<S - 2>();
           __syncwarp();        // block i of every lane is in; every lane is done with block i - 1
           issue(i + S - 1, (j + S - 1) % S);
-          const uint32_t at = ring + j * (2 * BT * HD);
+          const uint8_t* at = smem + warp * (S * 2 * BT * HD) + j * (2 * BT * HD);
           uint4 kr[4], vr[4];
           kr[0] = lds128(at + k_ld), kr[1] = lds128(at + (k_ld ^ 64));
           kr[2] = lds128(at + k_ld + 8 * HD), kr[3] = lds128(at + (k_ld ^ 64) + 8 * HD);

@@ -1,10 +1,9 @@
 // Products of a few rows with 4-bit weights: C[m][n] = sum_k x[m][k] (u[n][k] - 8) s[n][k / G] (+ bias), m < 64.
 //
-// Bound by the weight bytes (K N / 2) up to about 16 rows. The weights are the A operand of mma.m16n8k16 (16 columns of
-// B on the M side, up to 8 rows of x per n-tile), turned from 4 bits to bf16 in registers: the word's nibbles i and
-// i + 4 become the halves of one register, (w >> 4i) & 0x000F000F | 0x43004300 = 128 + u, minus 136, exact. A group's
-// products are summed by the tensor core in fp32 and scaled once as they are added to the fp32 result, so the only
-// rounding is the output's (and fp32's).
+// Bound by the weight bytes (K N / 2) at one row, by instruction issue from there on. The weights are the A operand of
+// mma.m16n8k16 (16 columns of B on the M side, up to 8 rows of x per n-tile), turned from 4 bits to bf16 in registers,
+// exactly (nibbles_lo). A group's products are summed by the tensor core in fp32 and scaled once as they are added to the
+// fp32 result, so the only rounding is the output's (and fp32's).
 //
 // Native layout, 0.5 byte a weight: tiles of 16 columns x 128 k, 1 KB, K running fastest. Lane 4g + c owns 16 bytes for
 // column g (first 512 bytes) and 16 for column g + 8; word q of them holds k = 32q + 8c .. + 7, nibble i the k 2i and
@@ -21,7 +20,6 @@ constexpr int TN = 16;          // columns per tile
 constexpr int TK = 128;         // k per tile
 constexpr int TILE = TN * TK / 2;
 constexpr int kMaxRows = 64;
-constexpr int kWarps = 8;
 
 __host__ __device__ inline int64_t tiles_n(int64_t N) { return (N + TN - 1) / TN; }
 __host__ __device__ inline int64_t tiles_k(int64_t K) { return (K + TK - 1) / TK; }
@@ -112,103 +110,324 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Nibbles i and i + 4 of a word as bf16 integers u - 8.
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) {
-  const uint32_t b = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+__device__ __forceinline__ void mma_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// Nibbles 0 and 4 (lo) or 1 and 5 (hi) of a word as bf16 values (u - 8) / 64. Taken as bf16 bits, a field in the low 8
+// bits is that integer times 2^-133 (subnormal, or the first binade, whose spacing is the same), so one FMA scales it and
+// takes the offset off, exactly. Three ALU instructions less per word than shifting every nibble to the same place and
+// setting an exponent beside it (the ALU pipe runs at half rate and was the busiest: 16.3 -> 13.3 us for 50 MB of codes).
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(b), "r"(0x43084308u));
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+__device__ __forceinline__ uint32_t nibbles_lo(uint32_t w) { return fma_bf16x2(w & 0x000F000Fu, 0x7F007F00u, 0xBE00BE00u); }
+__device__ __forceinline__ uint32_t nibbles_hi(uint32_t w) { return fma_bf16x2(w & 0x00F000F0u, 0x7D007D00u, 0xBE00BE00u); }
+constexpr float kUnit = 64.0f;   // what the sums are short of
 
-// One CTA per 16 columns: its warps take the k tiles in turn and are joined in shared memory in warp order.
-template <int NT, int G, bool kSwiglu>
-__global__ void __launch_bounds__(32 * kWarps) linear_kernel(const Args a) {
-  __shared__ float red[kWarps][8 * NT][TN + 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, c = lane & 3;
-  const int64_t kt = tiles_k(a.K);
-  const uint4* w = a.w + static_cast<int64_t>(blockIdx.x) * kt * (TILE / 16) + lane;
-  const uint32_t* sc = a.s + static_cast<int64_t>(blockIdx.x) * kt * (TK / G) * 8 + g;
-  float acc[NT][4];
+// A k tile's operands on their way: the lane's codes of columns g and g + 8 and the groups' scales.
+template <int G>
+struct Tile {
+  uint4 w0, w1;
+  uint32_t s[TK / G];
+};
+template <int G>
+__device__ __forceinline__ void load_tile(Tile<G>& t, const uint4* w, const uint32_t* sc) {
+  t.w0 = __ldcs(w), t.w1 = __ldcs(w + 32);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
-  for (int64_t t = warp; t < kt; t += kWarps) {
-    const uint4 w0 = __ldcs(w + t * (TILE / 16)), w1 = __ldcs(w + t * (TILE / 16) + 32);
-    const uint32_t v0[4] = {w0.x, w0.y, w0.z, w0.w}, v1[4] = {w1.x, w1.y, w1.z, w1.w};
-    float part[NT][4];
+  for (int j = 0; j < TK / G; ++j) t.s[j] = __ldcs(sc + j * 8);
+}
+
+// acc += the products of CT tiles with the same x fragments: x(q, nt) gives the 16 bytes of word q for row nt * 8 + g.
+template <int CT, int NT, int G, typename X>
+__device__ __forceinline__ void tile_product(const Tile<G> (&t)[CT], X x, float (&acc)[CT][NT][4]) {
+  float part[CT][NT][4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (q % (G / 32) == 0) {
+  for (int q = 0; q < 4; ++q) {
+    uint4 xv[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) part[nt][0] = part[nt][1] = part[nt][2] = part[nt][3] = 0.0f;
-      }
-      uint32_t A[8];
+    for (int nt = 0; nt < NT; ++nt) xv[nt] = x(q, nt);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) A[2 * i] = nibbles(v0[q], i), A[2 * i + 1] = nibbles(v1[q], i);
-      const int64_t k = t * TK + 32 * q + 8 * c;
+    for (int ct = 0; ct < CT; ++ct) {
+      const uint32_t v0 = q == 0 ? t[ct].w0.x : q == 1 ? t[ct].w0.y : q == 2 ? t[ct].w0.z : t[ct].w0.w;
+      const uint32_t v1 = q == 0 ? t[ct].w1.x : q == 1 ? t[ct].w1.y : q == 2 ? t[ct].w1.z : t[ct].w1.w;
+      const uint32_t h0 = v0 >> 8, h1 = v1 >> 8;
+      const uint32_t A[8] = {nibbles_lo(v0), nibbles_lo(v1), nibbles_hi(v0), nibbles_hi(v1),
+                             nibbles_lo(h0), nibbles_lo(h1), nibbles_hi(h0), nibbles_hi(h1)};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int m = nt * 8 + g;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (m < a.M && k < a.K) x = *reinterpret_cast<const uint4*>(a.x + m * a.K + k);
-        mma(part[nt], A[0], A[1], A[2], A[3], x.x, x.y);
-        mma(part[nt], A[4], A[5], A[6], A[7], x.z, x.w);
+        if (q % (G / 32) == 0) mma_zero(part[ct][nt], A[0], A[1], A[2], A[3], xv[nt].x, xv[nt].y);
+        else mma(part[ct][nt], A[0], A[1], A[2], A[3], xv[nt].x, xv[nt].y);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma(part[ct][nt], A[4], A[5], A[6], A[7], xv[nt].z, xv[nt].w);
       if (q % (G / 32) == G / 32 - 1) {
-        const uint32_t s = __ldg(sc + (t * (TK / G) + q / (G / 32)) * 8);
+        const uint32_t s = t[ct].s[q / (G / 32)];
         const float s0 = __uint_as_float(s << 16), s1 = __uint_as_float(s & 0xFFFF0000u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          acc[nt][0] = fmaf(s0, part[nt][0], acc[nt][0]);
-          acc[nt][1] = fmaf(s0, part[nt][1], acc[nt][1]);
-          acc[nt][2] = fmaf(s1, part[nt][2], acc[nt][2]);
-          acc[nt][3] = fmaf(s1, part[nt][3], acc[nt][3]);
+          acc[ct][nt][0] = fmaf(s0, part[ct][nt][0], acc[ct][nt][0]);
+          acc[ct][nt][1] = fmaf(s0, part[ct][nt][1], acc[ct][nt][1]);
+          acc[ct][nt][2] = fmaf(s1, part[ct][nt][2], acc[ct][nt][2]);
+          acc[ct][nt][3] = fmaf(s1, part[ct][nt][3], acc[ct][nt][3]);
         }
       }
     }
   }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][nt * 8 + 2 * c + (i & 1)][g + 8 * (i >> 1)] = acc[nt][i];
+}
+
+// Bias, activation and store of one output: v (and for SwiGLU the unit's projection) of row m, tile row r of tile t.
+template <bool kSwiglu>
+__device__ __forceinline__ void finish(const Args& a, int m, int64_t t, int r, float v, float up) {
+  const int64_t col = column_of(t, r, kSwiglu);
+  if (col >= a.N) return;
+  int64_t at = m * a.N + col;
+  if (a.bias) v += bf16_bits_to_float(a.bias[col]);
+  if (kSwiglu) {
+    if (a.bias) up += bf16_bits_to_float(a.bias[col + 64]);
+    v = v / (1.0f + __expf(-v)) * up;
+    at = m * (a.N / 2) + t * 8 + r;
   }
+  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+  else static_cast<uint16_t*>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+// Up to 8 rows: one CTA per 16 columns; its warps take the k tiles in turn, each with kDepth tiles on their way, and
+// are joined in shared memory in warp order. x comes straight from L1 and L2: it is small next to the weights. Lanes of
+// rows beyond M read the last row: a column of the B operand reaches its own column of the result only.
+constexpr int kFew = 8, kDepth = 2;
+template <int G, bool kSwiglu>
+__global__ void __launch_bounds__(32 * kFew, 4) few_kernel(const Args a) {
+  __shared__ float red[kFew][8][TN + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int K = static_cast<int>(a.K), kt = static_cast<int>(tiles_k(a.K));
+  constexpr int kSc = TK / G * 8;                                 // scale words of a tile
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kt + warp;
+  const uint4* w = a.w + at * (TILE / 16) + lane;
+  const uint32_t* sc = a.s + at * kSc + g;
+  const uint16_t* x = a.x + static_cast<int64_t>(min(g, a.M - 1)) * K + warp * TK + 8 * c;
+  const int n = kt > warp ? (kt - warp + kFew - 1) / kFew : 0;    // this warp's tiles
+  const int tail = K % TK != 0 && (kt - 1) % kFew == warp ? n - 1 : n;   // the one whose k ends inside it
+  float acc[1][1][4] = {{{0.0f, 0.0f, 0.0f, 0.0f}}};
+  Tile<G> ring[kDepth][1];
+#pragma unroll
+  for (int j = 0; j < kDepth; ++j)
+    if (j < n) load_tile<G>(ring[j][0], w + j * kFew * (TILE / 16), sc + j * kFew * kSc);
+  for (int t0 = 0; t0 < n; t0 += kDepth) {
+#pragma unroll
+    for (int j = 0; j < kDepth; ++j) {
+      if (t0 + j < n) {
+        uint4 xv[4];
+        if (t0 + j != tail) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) xv[q] = __ldg(reinterpret_cast<const uint4*>(x + j * kFew * TK + 32 * q));
+        } else {
+          const int left = K % TK - 8 * c;                        // k left of this lane's first
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            xv[q] = make_uint4(0, 0, 0, 0);
+            if (32 * q < left) xv[q] = __ldg(reinterpret_cast<const uint4*>(x + j * kFew * TK + 32 * q));
+          }
+        }
+        tile_product<1, 1, G>(ring[j], [&](int q, int) { return xv[q]; }, acc);
+        if (t0 + j + kDepth < n)
+          load_tile<G>(ring[j][0], w + (j + kDepth) * kFew * (TILE / 16), sc + (j + kDepth) * kFew * kSc);
+      }
+    }
+    x += kDepth * kFew * TK, w += kDepth * kFew * (TILE / 16), sc += kDepth * kFew * kSc;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[warp][2 * c + (i & 1)][g + 8 * (i >> 1)] = acc[0][0][i] * kUnit;
   __syncthreads();
   constexpr int kOut = kSwiglu ? 8 : TN;
-  for (int i = threadIdx.x; i < a.M * kOut; i += 32 * kWarps) {
+  for (int i = threadIdx.x; i < a.M * kOut; i += 32 * kFew) {
     const int m = i / kOut, r = i % kOut;
     float v = 0.0f, up = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
+    for (int k = 0; k < kFew; ++k) {
       v += red[k][m][r];
       if (kSwiglu) up += red[k][m][r + 8];
     }
-    const int64_t col = column_of(blockIdx.x, r, kSwiglu);
-    if (col >= a.N) continue;
-    int64_t at = m * a.N + col;
-    if (a.bias) v += bf16_bits_to_float(a.bias[col]);
-    if (kSwiglu) {
-      if (a.bias) up += bf16_bits_to_float(a.bias[col + 64]);
-      v = v / (1.0f + __expf(-v)) * up;
-      at = m * (a.N / 2) + static_cast<int64_t>(blockIdx.x) * 8 + r;
-    }
-    if (a.out_f32) static_cast<float*>(a.out)[at] = v;
-    else static_cast<uint16_t*>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    finish<kSwiglu>(a, m, blockIdx.x, r, v, up);
   }
 }
 
-template <int NT, int G>
-inline void launch(const Args& a, bool swiglu, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(tiles_n(a.N));
-  if (swiglu) linear_kernel<NT, G, true><<<grid, 32 * kWarps, 0, s>>>(a);
-  else linear_kernel<NT, G, false><<<grid, 32 * kWarps, 0, s>>>(a);
+// 9 to 64 rows: one CTA per 128 columns and share of K, a warp per CT x 16 columns; the x of a share is brought into
+// shared memory once (with one warp per 16 columns reading x itself, x is M / 8 times the weights' bytes of L2 traffic)
+// and each fragment serves CT tiles of codes. The CTAs of a cluster hold the shares of K of the same columns and are
+// joined through distributed shared memory in rank order.
+template <int NT>
+struct Many {
+  static constexpr int CT = NT <= 3 ? 2 : 1;
+  static constexpr int kCols = 128, kWarps = kCols / (CT * TN), kThreads = 32 * kWarps;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kX = kRows * TK * 2;                       // bytes of x per k tile
+  static constexpr int kCtas = NT <= 3 ? 3 : NT <= 4 ? 2 : 1;  // resident per SM
+  static constexpr int kDepth = 2;                                // k tiles of codes on their way
+  static constexpr int kPanel = 221184 / kCtas / kX / kDepth * kDepth;   // k tiles of x in shared memory at a time
+  static constexpr int kOut = kRows * (kCols + 4) * 4;            // this CTA's sums [row][column], padded
+  static constexpr int kSmem = kPanel * kX > kOut ? kPanel * kX : kOut;
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
 }
 
-template <int G>
-inline void launch_rows(const Args& a, bool swiglu, cudaStream_t s) {
-  if (a.M <= 8) launch<1, G>(a, swiglu, s);
-  else if (a.M <= 16) launch<2, G>(a, swiglu, s);
-  else if (a.M <= 32) launch<4, G>(a, swiglu, s);
-  else launch<8, G>(a, swiglu, s);
+template <int NT, int G, bool kSwiglu>
+__global__ void __launch_bounds__(Many<NT>::kThreads, Many<NT>::kCtas) many_kernel(const Args a, int shares, int log_shares) {
+  using C = Many<NT>;
+  constexpr int D = C::kDepth, CT = C::CT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int K = static_cast<int>(a.K), kt = static_cast<int>(tiles_k(a.K));
+  const int rank = blockIdx.x & (shares - 1);
+  const int64_t tile0 = static_cast<int64_t>(blockIdx.x >> log_shares) * (C::kCols / TN), tiles = tiles_n(a.N);
+  const int t_begin = (kt * rank) >> log_shares, t_end = (kt * (rank + 1)) >> log_shares;
+  constexpr int kSc = TK / G * 8;                                 // scale words of a tile
+  const uint4* w[CT];
+  const uint32_t* sc[CT];
+  Tile<G> ring[D][CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {                               // (a tile beyond the last is the last again, unused)
+    const int64_t at = min(tile0 + warp * CT + ct, tiles - 1) * kt + t_begin;
+    w[ct] = a.w + at * (TILE / 16) + lane;
+    sc[ct] = a.s + at * kSc + g;
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      if (t_begin + j < t_end) load_tile<G>(ring[j][ct], w[ct] + j * (TILE / 16), sc[ct] + j * kSc);
+  }
+  // Row m of a k tile keeps its 16-byte chunk j at chunk j ^ 4 (m & 1): the eight lanes of a phase (two rows, four
+  // chunks) then read eight different bank groups. A thread copies chunk tid % 16 of rows tid / 16, + kStep, ..; rows
+  // beyond M repeat the last (their results are not stored), k beyond K are zeros.
+  constexpr int kStep = C::kThreads / 16, kCopies = (C::kRows + kStep - 1) / kStep;
+  static_assert(kStep % 2 == 0, "rows of x per pass");
+  const int xm = threadIdx.x >> 4, xj = threadIdx.x & 15;
+  const uint32_t xdst = smem_u32(smem) + xm * (TK * 2) + ((xj ^ ((xm & 1) * 4)) << 4);
+  const uint16_t* xsrc[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i)
+    xsrc[i] = a.x + static_cast<int64_t>(min(xm + kStep * i, a.M - 1)) * K + t_begin * TK + 8 * xj;
+  float acc[CT][NT][4];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[ct][nt][0] = acc[ct][nt][1] = acc[ct][nt][2] = acc[ct][nt][3] = 0.0f;
+  const uint8_t* xa = smem + g * (TK * 2);
+  const uint32_t xc = (c ^ ((g & 1) * 4)) << 4;
+  for (int p0 = t_begin; p0 < t_end; p0 += C::kPanel) {           // (one panel, unless K is very long)
+    const int p1 = min(p0 + C::kPanel, t_end);
+    if (p0 > t_begin) __syncthreads();                            // every warp is done with the panel before
+    for (int t = p0; t < p1; ++t) {
+      const bool in = t * TK + 8 * xj < K;
+      const uint32_t dst = xdst + (t - p0) * C::kX;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        if (xm + kStep * i >= C::kRows) break;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * kStep * (TK * 2)),
+                     "l"(in ? xsrc[i] : a.x), "r"(in ? 16 : 0)
+                     : "memory");
+        xsrc[i] += TK;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    for (int t0 = p0; t0 < p1; t0 += D) {
+#pragma unroll
+      for (int j = 0; j < D; ++j) {
+        const int t = t0 + j;
+        if (t < p1) {
+          const uint8_t* at = xa + (t - p0) * C::kX;
+          tile_product<CT, NT, G>(ring[j], [&](int q, int nt) {
+            return *reinterpret_cast<const uint4*>(at + nt * 8 * (TK * 2) + (xc ^ (q << 6)));
+          }, acc);
+          if (t + D < t_end) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              load_tile<G>(ring[j][ct], w[ct] + (j + D) * (TILE / 16), sc[ct] + (j + D) * kSc);
+          }
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) w[ct] += D * (TILE / 16), sc[ct] += D * kSc;
+    }
+  }
+  __syncthreads();                                                // the panel becomes the sums
+  float* sums = reinterpret_cast<float*>(smem);
+  constexpr int kLd = C::kCols + 4;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sums[(nt * 8 + 2 * c + (i & 1)) * kLd + (warp * CT + ct) * TN + g + 8 * (i >> 1)] = acc[ct][nt][i] * kUnit;
+  if (shares > 1) cluster_sync(); else __syncthreads();
+  // this CTA finishes every shares-th (row, column) of the cluster's 128 columns
+  constexpr int kOut = kSwiglu ? C::kCols / 2 : C::kCols;
+  for (int i = threadIdx.x + rank * C::kThreads; i < a.M * kOut; i += C::kThreads << log_shares) {
+    const int m = i / kOut, n = i % kOut;
+    const int t = kSwiglu ? n >> 3 : n >> 4, r = kSwiglu ? n & 7 : n & 15;
+    const float* at = sums + m * kLd + t * TN + r;
+    float v = 0.0f, up = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < shares; ++k) {
+      const uint32_t remote = mapa_shared(smem_u32(at), k);
+      v += ld_cluster(remote);
+      if (kSwiglu) up += ld_cluster(remote + 32);
+    }
+    if (tile0 + t < tiles) finish<kSwiglu>(a, m, tile0 + t, r, v, up);
+  }
+  if (shares > 1) cluster_sync();                                 // no CTA leaves while its sums are read
+}
+
+template <int NT, int G, bool kSwiglu>
+inline int launch_many(const Args& a, cudaStream_t s) {
+  auto kern = many_kernel<NT, G, kSwiglu>;
+  RL_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<NT>::kSmem));
+  // shares of K: as many as keep the grid within the GPU's resident CTAs and leave each at least two k tiles
+  const int64_t groups = (a.N + Many<NT>::kCols - 1) / Many<NT>::kCols, kt = tiles_k(a.K);
+  const int64_t slots = static_cast<int64_t>(sm_count()) * Many<NT>::kCtas;
+  int log_shares = 0;
+  while (log_shares < 3 && (groups << (log_shares + 1)) <= slots && kt >= (4 << log_shares)) ++log_shares;
+  const int shares = 1 << log_shares;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * shares));
+  cfg.blockDim = dim3(Many<NT>::kThreads);
+  cfg.dynamicSmemBytes = Many<NT>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = shares;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  RL_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, a, shares, log_shares));
+  return RL_OK;
+}
+
+template <int G, bool kSwiglu>
+inline int launch(const Args& a, cudaStream_t s) {
+  if (a.M <= 8) {
+    few_kernel<G, kSwiglu><<<static_cast<unsigned>(tiles_n(a.N)), 32 * kFew, 0, s>>>(a);
+    RL_TRY_CUDA(cudaGetLastError());
+    return RL_OK;
+  }
+  switch ((a.M + 7) / 8) {
+    case 2: return launch_many<2, G, kSwiglu>(a, s);
+    case 3: return launch_many<3, G, kSwiglu>(a, s);
+    case 4: return launch_many<4, G, kSwiglu>(a, s);
+    case 5:
+    case 6: return launch_many<6, G, kSwiglu>(a, s);
+    default: return launch_many<8, G, kSwiglu>(a, s);
+  }
 }
 
 inline int check_shape(const char* fn, int64_t K, int64_t N, int group, int swiglu) {
@@ -298,12 +517,10 @@ int rl_linear_w4(const uint16_t* x, int64_t M, int64_t K, const uint8_t* w, cons
   const w4::Args a{x, reinterpret_cast<const uint4*>(w), reinterpret_cast<const uint32_t*>(scales),
                    epilogue == RL_EPI_NONE ? nullptr : bias, out, K, N, static_cast<int>(M), out_dtype == RL_F32};
   switch (group) {
-    case 32: w4::launch_rows<32>(a, swiglu, stream); break;
-    case 64: w4::launch_rows<64>(a, swiglu, stream); break;
-    default: w4::launch_rows<128>(a, swiglu, stream); break;
+    case 32: return swiglu ? w4::launch<32, true>(a, stream) : w4::launch<32, false>(a, stream);
+    case 64: return swiglu ? w4::launch<64, true>(a, stream) : w4::launch<64, false>(a, stream);
+    default: return swiglu ? w4::launch<128, true>(a, stream) : w4::launch<128, false>(a, stream);
   }
-  RL_TRY_CUDA(cudaGetLastError());
-  return RL_OK;
 }
 
 }  // extern "C"
