@@ -425,6 +425,10 @@ int rl_kv_read(const uint8_t* pool_k, const uint8_t* pool_v, const uint8_t* pool
 int rl_kv_copy_pages(uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke, uint8_t* pool_ve, int layers, int64_t pages,
                      int kv_heads, int page, const int32_t* src, const int32_t* dst, int64_t n, rl_stream_t stream);
 
+/* dst[at[i]] = value[i] for i < n: host arrays, read before the call returns, each entry of `at` once and below `size`.
+ * Page tables and lengths in device memory follow the host's bookkeeping by this call. */
+int rl_kv_set(int32_t* dst, int64_t size, const int32_t* at, const int32_t* value, int64_t n, rl_stream_t stream);
+
 /*
  * Attention of the new tokens over the cache (grouped-query: query head h reads K/V head h / (heads / kv_heads)).
  * q: bf16, element (row, head, dim) at row * q_st + head * q_sh + dim, strides multiples of 8, 16-byte aligned.

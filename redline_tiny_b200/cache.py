@@ -1,0 +1,213 @@
+"""The pages of an 8-bit cache of keys and values, and the sequences that live in them.
+
+`PagedKV` owns a pool (ops.KVPool) and keeps its books on the host: which pages a sequence has, how many sequences share a
+page, which are free. Forking a sequence copies nothing; a page that several sequences share is copied when one of them
+first writes into it, all such copies of a step in one launch. Batches carry the page tables and lengths in device memory
+at fixed addresses, so a captured decode step follows them when it is replayed.
+
+    kv = PagedKV(layers=36, pages=4096, kv_heads=8)
+    a = kv.new()
+    batch = kv.batch([a])
+    batch.extend([len(prompt)])                 # pages for the new tokens; raises (and changes nothing) without room
+    ops.kv_append(kv.pool, layer, k, v, *batch.args)
+    o = ops.kv_attention(q, kv.pool, layer, *batch.args)
+    b = kv.fork(a)                              # b continues where a stands
+    kv.free(a)
+"""
+
+import heapq
+
+import torch
+
+from . import ops
+
+
+class OutOfPages(RuntimeError):
+    """The pool has fewer free pages than a step needs; nothing was changed."""
+
+
+class PagedKV:
+    def __init__(self, layers, pages, kv_heads, page=64, device="cuda"):
+        self.pool = ops.KVPool.empty(layers, pages, kv_heads, page, device)
+        self.page = page
+        self.refs = [0] * pages            # sequences that hold the page
+        self._free = list(range(pages))    # a heap: the lowest page is taken first
+        self._seqs = {}                    # sequence -> its pages in order
+        self._len = {}
+        self._next = 0
+
+    # -- books ------------------------------------------------------------------------------------------------------
+    def new(self):
+        """An empty sequence."""
+        s = self._next
+        self._next += 1
+        self._seqs[s], self._len[s] = [], 0
+        return s
+
+    def fork(self, seq):
+        """A sequence that continues where `seq` stands, sharing all its pages."""
+        length, pages = self.length(seq), self._seqs[seq]
+        s = self.new()
+        self._seqs[s], self._len[s] = list(pages), length
+        for p in pages:
+            self.refs[p] += 1
+        return s
+
+    def free(self, seq):
+        """Give up a sequence; pages that no other sequence holds are free again."""
+        self.length(seq)
+        self._release(self._seqs.pop(seq))
+        del self._len[seq]
+
+    def truncate(self, seq, length):
+        """Forget the tokens from position `length` on."""
+        if not 0 <= length <= self.length(seq):
+            raise ValueError(f"sequence {seq} has {self._len[seq]} tokens")
+        pages, keep = self._seqs[seq], -(-length // self.page)
+        self._release(pages[keep:])
+        del pages[keep:]
+        self._len[seq] = length
+
+    def _release(self, pages):
+        for p in pages:
+            self.refs[p] -= 1
+            if self.refs[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def length(self, seq):
+        if seq not in self._len:
+            raise ValueError(f"no sequence {seq} in this cache")
+        return self._len[seq]
+
+    def pages(self, seq):
+        return tuple(self._seqs[seq])
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    # -- steps ------------------------------------------------------------------------------------------------------
+    def batch(self, seqs, max_pages=None):
+        """A batch of different sequences; `max_pages` bounds the pages of each (default: the whole pool)."""
+        return Batch(self, seqs, max_pages or len(self.refs))
+
+    def _extend(self, seqs, counts):
+        """Room for counts[i] more tokens of seqs[i]: (page, its private copy) pairs to copy."""
+        fresh, shared = 0, {}
+        for s, n in zip(seqs, counts):
+            if n < 0:
+                raise ValueError(f"{n} new tokens")
+            have, pages = self._len[s], self._seqs[s]
+            fresh += -(-(have + n) // self.page) - len(pages)
+            if n and have % self.page and self.refs[pages[-1]] > 1:   # the page it continues in is shared
+                p = pages[-1]
+                shared[p] = shared.get(p, 0) + 1
+        # the last holder of a page keeps it when every holder writes into it
+        copies_needed = sum(min(c, self.refs[p] - 1) for p, c in shared.items())
+        if fresh + copies_needed > len(self._free):
+            raise OutOfPages(f"{fresh + copies_needed} pages needed, {len(self._free)} free")
+        copies = []
+        for s, n in zip(seqs, counts):
+            have, pages = self._len[s], self._seqs[s]
+            if n and have % self.page and self.refs[pages[-1]] > 1:
+                p, q = pages[-1], heapq.heappop(self._free)
+                self.refs[p] -= 1
+                self.refs[q] = 1
+                pages[-1] = q
+                copies.append((p, q))
+            for _ in range(-(-(have + n) // self.page) - len(pages)):
+                q = heapq.heappop(self._free)
+                self.refs[q] = 1
+                pages.append(q)
+            self._len[s] = have + n
+        return copies
+
+    def compact(self):
+        """Move the live pages to the front of the pool, so that its tail can be given back (resize). Returns the number
+        of pages moved. A batch follows at its next `extend` (of no tokens, if need be), not before."""
+        live = [p for p, r in enumerate(self.refs) if r]
+        n = len(live)
+        to = dict(zip([p for p in live if p >= n], [p for p in range(n) if not self.refs[p]]))
+        if to:
+            ops.kv_copy_pages(self.pool, list(to.keys()), list(to.values()))
+            for p, q in to.items():
+                self.refs[q], self.refs[p] = self.refs[p], 0
+            for pages in self._seqs.values():
+                pages[:] = [to.get(p, p) for p in pages]
+            self._free = list(range(n, len(self.refs)))
+        return len(to)
+
+    def resize(self, pages):
+        """A pool of `pages` pages (compacted first when that drops any). Captured graphs hold the old one."""
+        if pages < len(self.refs):
+            if pages < sum(1 for r in self.refs if r):
+                raise OutOfPages(f"{sum(1 for r in self.refs if r)} pages are in use")
+            self.compact()
+        old, n = self.pool, min(pages, len(self.refs))
+        self.pool = ops.KVPool.empty(old.layers, pages, old.kv_heads, old.page, old.k.device)
+        for a, b in zip((self.pool.k, self.pool.v, self.pool.k_exp, self.pool.v_exp),
+                        (old.k, old.v, old.k_exp, old.v_exp)):
+            a[:, :n].copy_(b[:, :n])
+        self.refs = self.refs[:pages] + [0] * (pages - len(self.refs))
+        self._free = [p for p, r in enumerate(self.refs) if not r]
+
+
+class Batch:
+    """Sequences that take steps together. `args` = (table, kv_len, q_start): the device arrays that ops.kv_append and
+    ops.kv_attention take, at addresses that never change."""
+
+    def __init__(self, kv, seqs, max_pages):
+        self.kv, self.seqs = kv, list(seqs)
+        if len(set(self.seqs)) != len(self.seqs):
+            raise ValueError("a sequence appears twice in a batch")
+        for s in self.seqs:
+            kv.length(s)
+        B, self.width = len(self.seqs), int(max_pages)
+        dev = kv.pool.k.device
+        self._meta = torch.full((B * self.width + 2 * B + 1,), -1, dtype=torch.int32, device=dev)
+        self._meta[B * self.width:] = 0
+        self._written = [[] for _ in self.seqs]      # what the device tables hold
+        self._lens, self._starts = [0] * B, [0] * (B + 1)
+        self.table = self._meta[:B * self.width].view(B, self.width)
+        self.kv_len = self._meta[B * self.width:B * self.width + B]
+        self.q_start = self._meta[B * self.width + B:]
+
+    @property
+    def args(self):
+        return self.table, self.kv_len, self.q_start
+
+    def extend(self, counts):
+        """Make room for counts[i] new tokens of each sequence and point the device arrays at them: pages are taken,
+        shared pages that will be written are copied. Raises OutOfPages, with nothing changed, where the pool is full."""
+        counts = list(counts)
+        kv, B = self.kv, len(self.seqs)
+        if len(counts) != B:
+            raise ValueError(f"{len(counts)} counts for {B} sequences")
+        for s, n in zip(self.seqs, counts):
+            need = -(-(kv.length(s) + n) // kv.page)
+            if need > len(kv.refs):
+                raise OutOfPages(f"sequence {s} needs {need} pages of a pool of {len(kv.refs)}")
+            if need > self.width:
+                raise ValueError(f"sequence {s} would need more than the batch's {self.width} pages a sequence")
+        copies = kv._extend(self.seqs, counts)
+        if copies:
+            ops.kv_copy_pages(kv.pool, [a for a, _ in copies], [b for _, b in copies])
+        self._write(counts)
+
+    def _write(self, counts):
+        kv, B, W, new = self.kv, len(self.seqs), self.width, {}
+        for b, s in enumerate(self.seqs):
+            pages, have = kv._seqs[s], self._written[b]
+            for i, p in enumerate(pages):
+                if i >= len(have) or have[i] != p:
+                    new[b * W + i] = p
+            self._written[b] = list(pages)
+            if self._lens[b] != kv.length(s):
+                self._lens[b] = new[B * W + b] = kv.length(s)
+        at = 0
+        for b in range(B + 1):
+            if self._starts[b] != at:
+                self._starts[b] = new[B * W + B + b] = at
+            at += counts[b] if b < B else 0
+        if new:
+            ops.kv_set(self._meta, new)

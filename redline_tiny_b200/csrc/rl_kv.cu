@@ -274,6 +274,14 @@ __global__ void __launch_bounds__(256) copy_kernel(const Pool p, int64_t layer_c
   }
 }
 
+// dst[at[i]] = value[i]: page tables and lengths follow the host's bookkeeping without a host-to-device copy, whose source
+// the caller would have to keep unchanged until it ran.
+template <int N>
+__global__ void __launch_bounds__(N < 1024 ? N : 1024) set_kernel(int32_t* dst, int n, const __grid_constant__ Pairs<N> p) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) dst[p.src[i]] = p.dst[i];
+}
+
 inline int check_pool(const char* fn, const Pool& p) {
   RL_REQUIRE(p.k && p.v && p.ke && p.ve, RL_ERR_ARGUMENT, "%s: NULL pool pointer", fn);
   RL_REQUIRE(p.hkv > 0 && p.hkv <= 65535 && p.pages > 0 && p.pages <= INT32_MAX, RL_ERR_ARGUMENT,
@@ -397,6 +405,33 @@ int rl_kv_copy_pages(uint8_t* pool_k, uint8_t* pool_v, uint8_t* pool_ke, uint8_t
     st = m <= 32 ? kv::copy_launch<32>(p, layers, lc, le, src + i, dst + i, m, stream)
                  : kv::copy_launch<1024>(p, layers, lc, le, src + i, dst + i, m, stream);
     if (st != RL_OK) return st;
+  }
+  return RL_OK;
+}
+
+int rl_kv_set(int32_t* dst, int64_t size, const int32_t* at, const int32_t* value, int64_t n, rl_stream_t stream) {
+  using namespace rl;
+  RL_REQUIRE(n >= 0 && size >= 0 && size <= INT32_MAX, RL_ERR_ARGUMENT, "rl_kv_set: %lld entries of %lld", (long long)n,
+             (long long)size);
+  if (n == 0) return RL_OK;
+  RL_REQUIRE(dst && at && value, RL_ERR_ARGUMENT, "rl_kv_set: NULL pointer");
+  RL_REQUIRE(aligned(dst, 4), RL_ERR_ALIGNMENT, "rl_kv_set: dst must be 4-byte aligned");
+  for (int64_t i = 0; i < n; ++i)
+    RL_REQUIRE(at[i] >= 0 && at[i] < size, RL_ERR_ARGUMENT, "rl_kv_set: entry %d of an array of %lld", at[i],
+               (long long)size);
+  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_set: needs an sm_100 device");
+  for (int64_t i = 0; i < n; i += 1024) {
+    const int m = static_cast<int>(n - i < 1024 ? n - i : 1024);
+    if (m <= 256) {
+      kv::Pairs<256> a = {};
+      for (int j = 0; j < m; ++j) a.src[j] = at[i + j], a.dst[j] = value[i + j];
+      kv::set_kernel<256><<<1, 256, 0, stream>>>(dst, m, a);
+    } else {
+      kv::Pairs<1024> a = {};
+      for (int j = 0; j < m; ++j) a.src[j] = at[i + j], a.dst[j] = value[i + j];
+      kv::set_kernel<1024><<<1, 1024, 0, stream>>>(dst, m, a);
+    }
+    RL_TRY_CUDA(cudaGetLastError());
   }
   return RL_OK;
 }

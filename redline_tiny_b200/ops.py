@@ -12,7 +12,7 @@ through its C ABI on the current torch stream.
 
 Continuing sequences token by token (no counterpart in the reference):
 
-  KVPool, kv_append, kv_read, kv_copy_pages, kv_attention   the 8-bit paged cache (cache.PagedKV manages its pages)
+  KVPool, kv_append, kv_read, kv_copy_pages, kv_set, kv_attention   the 8-bit paged cache (cache.PagedKV keeps its pages)
   Weight4, linear_w4, swiglu_w4                             products of up to 64 rows with 4-bit weights
 """
 
@@ -408,6 +408,16 @@ def kv_copy_pages(pool, src, dst):
         raise ValueError(f"{len(a)} source pages for {len(b)} destinations")
     L.call("rl_kv_copy_pages", *pool._ptrs[0], pool.layers, pool.pages, pool.kv_heads, pool.page, a.buffer_info()[0],
            b.buffer_info()[0], len(a), _stream_of(dev))
+
+
+def kv_set(t, entries):
+    """t.view(-1)[i] = value for the items of `entries` (a dict on the host) of a contiguous int32 tensor, in stream
+    order, without a copy from host memory."""
+    dev = _here(t)
+    if t.dtype is not torch.int32 or not t.is_contiguous():
+        raise ValueError("kv_set takes a contiguous int32 tensor")
+    at, value = array.array("i", entries.keys()), array.array("i", entries.values())
+    L.call("rl_kv_set", t.data_ptr(), t.numel(), at.buffer_info()[0], value.buffer_info()[0], len(at), _stream_of(dev))
 
 
 @functools.lru_cache(maxsize=4096)

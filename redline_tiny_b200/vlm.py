@@ -153,3 +153,56 @@ class LM:
         x0, x1 = self.x[self.cur], self.x[(self.cur + 1) % 3]
         self._rms(x0, self.br, self.layers[-1]["p_in"], x1, self.a)
         return x1
+
+
+class CachedLM:
+    """The decoder layers over an 8-bit paged cache (cache.PagedKV), for sequences that go on token by token.
+
+    forward() takes the new rows of a batch: up to `few` (at most 64) of them run through 4-bit weights (ops.Weight4,
+    group scales; the products of a decode step are bound by weight bytes), more through the packed bfp16 GEMMs, and
+    both attend over the cache that they append to. Layer weights as LM's; few = 0 leaves the 4-bit form out."""
+
+    def __init__(self, cfg, weights, kv, few=64, group=64, device="cuda"):
+        if not 0 <= few <= 64:
+            raise ValueError("the 4-bit products take up to 64 rows")
+        if (kv.pool.layers, kv.pool.kv_heads) != (cfg.layers, cfg.kv_heads):
+            raise ValueError(f"the cache has {kv.pool.layers} layers of {kv.pool.kv_heads} K/V heads, the model "
+                             f"{cfg.layers} of {cfg.kv_heads}")
+        self.cfg, self.kv, self.few = cfg, kv, few
+        self.layers = []
+        for lw in weights["layers"]:
+            up = interleave_up_torch(lw["gate"], lw["up"]).to(device)
+            mats = {"qkv": lw["qkv"].to(device), "o": lw["o"].to(device), "up": up, "down": lw["down"].to(device)}
+            self.layers.append({
+                "w4": {n: ops.Weight4.from_float(m, group, swiglu=n == "up") for n, m in mats.items()} if few else None,
+                "bfp": {n: ops.PackedWeight.from_float(m, swiglu=n == "up") for n, m in mats.items()},
+                "p_in": rms_params(lw["w_in"].to(device)), "p_post": rms_params(lw["w_post"].to(device)),
+                "wq": (lw["q_norm"] * C_LOG2).to(device).float().contiguous(),
+                "wk": lw["k_norm"].to(device).float().contiguous(),
+            })
+
+    def forward(self, x, batch, cos, sin):
+        """x (T, hidden) bf16: the rows of the new tokens of batch.extend(counts), sequence by sequence; cos, sin
+        (T, 64): the RoPE rows of their positions. Appends their keys and values to every layer's cache and returns the
+        residual stream after the last layer, bf16 (T, hidden)."""
+        cfg, T = self.cfg, x.shape[0]
+        if T == 0:
+            return x
+        rope = torch.stack([cos.float(), sin.float()], -1).reshape(T, 128).contiguous()
+        x, branch = x.contiguous(), None
+        for i, lw in enumerate(self.layers):
+            x, a, _ = ops.ln_mod(x, branch, lw["p_in"], rms=True)
+            q, k, vt = ops.qkv_post(self._linear(a, lw, "qkv"), rope, lw["wq"], lw["wk"], cfg.heads, kv_heads=cfg.kv_heads)
+            ops.kv_append(self.kv.pool, i, k.transpose(0, 1), vt.permute(2, 0, 1)[:T], *batch.args)
+            o = ops.kv_attention(q.transpose(0, 1), self.kv.pool, i, *batch.args, scale_log2=1.0)
+            x, a, _ = ops.ln_mod(x, self._linear(o, lw, "o", raw=True), lw["p_post"], rms=True)
+            h = ops.swiglu_w4(a, lw["w4"]["up"]) if T <= self.few else ops.swiglu_up(a, lw["bfp"]["up"])
+            branch = self._linear(h, lw, "down")
+        return ops.ln_mod(x, branch, self.layers[-1]["p_in"], rms=True)[0]
+
+    def _linear(self, a, lw, name, raw=False):
+        if a.shape[0] <= self.few:
+            return ops.linear_w4(a, lw["w4"][name])
+        if raw:   # the bfp16 GEMM takes bfp16 values
+            a = ops.quantize_bfp16(a, want_bytes=False)[1]
+        return ops.linear_bfp16(a, lw["bfp"][name])
