@@ -75,6 +75,7 @@ SIGNATURES = {
     "rl_kv_read": (_I, [_P, _P, _P, _P, _I64, _I, _I, _P, _I64, _P, _P, _I, _I64, _P, _P, _P]),
     "rl_kv_copy_pages": (_I, [_P, _P, _P, _P, _I, _I64, _I, _I, _P, _P, _I64, _P]),
     "rl_kv_set": (_I, [_P, _I64, _P, _P, _I64, _P]),
+    "rl_set_kv_attention_path": (_I, [_I]),
     "rl_kv_attention_workspace": (ctypes.c_size_t, [_I64, _I, _I, _I]),
     "rl_kv_attention": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _I, _P, _I64, _P, _P, _I, _P,
                              ctypes.c_float, _P, _I64, _P, ctypes.c_size_t, _P]),

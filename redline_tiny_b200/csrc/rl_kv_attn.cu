@@ -672,60 +672,3 @@ inline int launch(const Args& a, cudaStream_t st) {
 
 }  // namespace kvattn
 }  // namespace rl
-
-extern "C" {
-
-size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads) {
-  using namespace rl;
-  if (T <= 0 || B <= 0 || kv_heads <= 0 || heads <= 0) return 0;
-  const int nt = kvattn::tile_n(T, B, heads / kv_heads);
-  return kvattn::part_bytes(nt) + static_cast<size_t>(kvattn::ctas_of(nt)) * sizeof(kvattn::Record);
-}
-
-int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, int heads, const uint8_t* pool_k,
-                    const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve, int64_t pages, int kv_heads,
-                    int page, const int32_t* table, int64_t table_ld, const int32_t* kv_len, const int32_t* q_start,
-                    int B, const int32_t* row_limit, float scale_log2, uint16_t* o, int64_t ldo, void* workspace,
-                    size_t workspace_bytes, rl_stream_t stream) {
-  using namespace rl;
-  kvattn::Args a;
-  a.pool = kv::Pool{const_cast<uint8_t*>(pool_k), const_cast<uint8_t*>(pool_v), const_cast<uint8_t*>(pool_ke),
-                    const_cast<uint8_t*>(pool_ve), pages, kv_heads, page};
-  a.batch = kv::Batch{table, table_ld, kv_len, q_start, B, T};
-  int st;
-  if ((st = kv::check_pool("rl_kv_attention", a.pool)) != RL_OK ||
-      (st = kv::check_batch("rl_kv_attention", a.batch)) != RL_OK)
-    return st;
-  RL_REQUIRE(heads > 0 && heads % kv_heads == 0, RL_ERR_ARGUMENT, "rl_kv_attention: %d query heads over %d K/V heads",
-             heads, kv_heads);
-  RL_REQUIRE(pages * kv_heads * (page / kv::BT) <= INT32_MAX, RL_ERR_ARGUMENT, "rl_kv_attention: %lld pages",
-             (long long)pages);
-  RL_REQUIRE(T * heads < (1ll << 31), RL_ERR_ARGUMENT, "rl_kv_attention: %lld rows of %d heads", (long long)T, heads);
-  RL_REQUIRE(table_ld * page <= (1 << 30), RL_ERR_ARGUMENT, "rl_kv_attention: sequences of up to %lld tokens",
-             (long long)(table_ld * page));
-  if (T == 0 || B == 0) return RL_OK;
-  RL_REQUIRE(q && q_start && o, RL_ERR_ARGUMENT, "rl_kv_attention: NULL pointer");
-  RL_REQUIRE(aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0 && aligned(o, 2) && aligned(row_limit, 4), RL_ERR_ALIGNMENT,
-             "rl_kv_attention: q must be 16-byte aligned, its strides multiples of 8");
-  RL_REQUIRE(ldo >= static_cast<int64_t>(heads) * kv::HD, RL_ERR_ARGUMENT, "rl_kv_attention: ldo < heads * 128");
-  const size_t need = rl_kv_attention_workspace(T, B, heads, kv_heads);
-  RL_REQUIRE(workspace && workspace_bytes >= need, RL_ERR_ARGUMENT, "rl_kv_attention: workspace of %zu bytes, needs %zu",
-             workspace_bytes, need);
-  RL_REQUIRE(aligned(workspace, 16), RL_ERR_ALIGNMENT, "rl_kv_attention: the workspace must be 16-byte aligned");
-  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_attention: needs an sm_100 device");
-  a.q = q, a.q_st = q_st, a.q_sh = q_sh;
-  a.row_limit = row_limit, a.scale_log2 = scale_log2;
-  a.o = o, a.ldo = ldo;
-  a.group = kvattn::Div::of(heads / kv_heads), a.hkv = kvattn::Div::of(kv_heads);
-  a.page_sh = __builtin_ctz(page);
-  const int nt = kvattn::tile_n(T, B, heads / kv_heads);
-  a.part = static_cast<float*>(workspace);
-  a.rec = reinterpret_cast<kvattn::Record*>(static_cast<uint8_t*>(workspace) + kvattn::part_bytes(nt));
-  switch (nt) {
-    case 1: return kvattn::launch<1>(a, stream);
-    case 2: return kvattn::launch<2>(a, stream);
-    default: return kvattn::launch<4>(a, stream);
-  }
-}
-
-}  // extern "C"

@@ -1,0 +1,97 @@
+// C ABI of the attention over the paged cache: the choice between the split kernel (rl_kv_attn.cu) and the prompt kernel
+// (rl_kv_prompt.cu).
+#include "rl_common.cuh"
+#include "rl_host.h"
+
+namespace rl {
+namespace kvattn {
+
+inline int& path() {   // 0 = by the rule below, 1 = split kernel, 2 = prompt kernel
+  static int v = 0;
+  return v;
+}
+
+// The prompt kernel computes 256 rows x 128 keys in the time in which the split kernel, which runs on every SM whatever
+// the shape, gets through about a quarter of them: it pays where its tiles are more than a quarter full of rows and
+// the SMs more than a quarter full of tiles. (It scales row maxima, so it takes positive scales.)
+inline bool by_prompt(int64_t T, int B, int heads, int kv_heads, float scale_log2) {
+  if (!(scale_log2 > 0.0f) || path() == 1) return false;
+  if (path() == 2) return true;
+  const int64_t rows = T * (heads / kv_heads), each = (rows + B - 1) / B;
+  const int64_t tiles = (each + kvprompt::ROWS - 1) / kvprompt::ROWS * B;
+  const double full = static_cast<double>(rows) / (static_cast<double>(tiles) * kvprompt::ROWS);
+  const double busy = static_cast<double>(tiles * kv_heads) / sm_count();
+  return full * (busy < 1.0 ? busy : 1.0) > 0.25;
+}
+
+}  // namespace kvattn
+}  // namespace rl
+
+extern "C" {
+
+int rl_set_kv_attention_path(int path) {
+  const int prev = rl::kvattn::path();
+  rl::kvattn::path() = path;
+  return prev;
+}
+
+size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads) {
+  using namespace rl;
+  if (T <= 0 || B <= 0 || kv_heads <= 0 || heads <= 0) return 0;
+  const int nt = kvattn::tile_n(T, B, heads / kv_heads);
+  return kvattn::part_bytes(nt) + static_cast<size_t>(kvattn::ctas_of(nt)) * sizeof(kvattn::Record);
+}
+
+int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, int heads, const uint8_t* pool_k,
+                    const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve, int64_t pages, int kv_heads,
+                    int page, const int32_t* table, int64_t table_ld, const int32_t* kv_len, const int32_t* q_start,
+                    int B, const int32_t* row_limit, float scale_log2, uint16_t* o, int64_t ldo, void* workspace,
+                    size_t workspace_bytes, rl_stream_t stream) {
+  using namespace rl;
+  kvattn::Args a;
+  a.pool = kv::Pool{const_cast<uint8_t*>(pool_k), const_cast<uint8_t*>(pool_v), const_cast<uint8_t*>(pool_ke),
+                    const_cast<uint8_t*>(pool_ve), pages, kv_heads, page};
+  a.batch = kv::Batch{table, table_ld, kv_len, q_start, B, T};
+  int st;
+  if ((st = kv::check_pool("rl_kv_attention", a.pool)) != RL_OK ||
+      (st = kv::check_batch("rl_kv_attention", a.batch)) != RL_OK)
+    return st;
+  RL_REQUIRE(heads > 0 && heads % kv_heads == 0, RL_ERR_ARGUMENT, "rl_kv_attention: %d query heads over %d K/V heads",
+             heads, kv_heads);
+  RL_REQUIRE(pages * kv_heads * (page / kv::BT) <= INT32_MAX, RL_ERR_ARGUMENT, "rl_kv_attention: %lld pages",
+             (long long)pages);
+  RL_REQUIRE(T * heads < (1ll << 31), RL_ERR_ARGUMENT, "rl_kv_attention: %lld rows of %d heads", (long long)T, heads);
+  RL_REQUIRE(table_ld * page <= (1 << 30), RL_ERR_ARGUMENT, "rl_kv_attention: sequences of up to %lld tokens",
+             (long long)(table_ld * page));
+  if (T == 0 || B == 0) return RL_OK;
+  RL_REQUIRE(q && q_start && o, RL_ERR_ARGUMENT, "rl_kv_attention: NULL pointer");
+  RL_REQUIRE(aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0 && aligned(o, 2) && aligned(row_limit, 4), RL_ERR_ALIGNMENT,
+             "rl_kv_attention: q must be 16-byte aligned, its strides multiples of 8");
+  RL_REQUIRE(ldo >= static_cast<int64_t>(heads) * kv::HD, RL_ERR_ARGUMENT, "rl_kv_attention: ldo < heads * 128");
+  const size_t need = rl_kv_attention_workspace(T, B, heads, kv_heads);
+  RL_REQUIRE(workspace && workspace_bytes >= need, RL_ERR_ARGUMENT, "rl_kv_attention: workspace of %zu bytes, needs %zu",
+             workspace_bytes, need);
+  RL_REQUIRE(aligned(workspace, 16), RL_ERR_ALIGNMENT, "rl_kv_attention: the workspace must be 16-byte aligned");
+  RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_attention: needs an sm_100 device");
+  a.q = q, a.q_st = q_st, a.q_sh = q_sh;
+  a.row_limit = row_limit, a.scale_log2 = scale_log2;
+  a.o = o, a.ldo = ldo;
+  a.group = kvattn::Div::of(heads / kv_heads), a.hkv = kvattn::Div::of(kv_heads);
+  a.page_sh = __builtin_ctz(page);
+  if (kvattn::by_prompt(T, B, heads, kv_heads, scale_log2)) {
+    const kvprompt::Args p{q, q_st, q_sh, a.pool, a.batch, row_limit, scale_log2, o, ldo, a.group, a.hkv, a.page_sh,
+                           aligned(o, 16) && ldo % 8 == 0};
+    // at most this many: a sequence's last tile of 256 rows may be a part
+    return kvprompt::launch((T * (heads / kv_heads) / kvprompt::ROWS + B) * kv_heads, p, stream);
+  }
+  const int nt = kvattn::tile_n(T, B, heads / kv_heads);
+  a.part = static_cast<float*>(workspace);
+  a.rec = reinterpret_cast<kvattn::Record*>(static_cast<uint8_t*>(workspace) + kvattn::part_bytes(nt));
+  switch (nt) {
+    case 1: return kvattn::launch<1>(a, stream);
+    case 2: return kvattn::launch<2>(a, stream);
+    default: return kvattn::launch<4>(a, stream);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,536 @@
+// Attention of many new tokens per sequence (prompts and their chunks) over the 8-bit paged cache, on tcgen05.
+//
+// One CTA per 256 rows (two 128-row tiles; rows = new tokens x query heads of one K/V head, token-major) of one
+// sequence, over 128-key blocks, with the schedule of the dense two-tile attention kernel (rl_attn.cu): per block and
+// tile S_t = Q_t K^T (M128 N128, bf16) into TMEM, softmax of one row per thread, P written back over S_t, and
+// O_t += P_t V, the two tiles interleaved so that one's MMAs run under the other's softmax. What differs is the operands:
+//
+//  * three converter warps read the pages' codes and write the MMA operands into shared memory. K: bf16 (u - 128) / 64,
+//    exact (a byte taken as bf16 bits is u 2^-133, so one FMA scales it and takes the offset off); the block's scale
+//    2^(ek - 133) is applied to S, 16 columns at a time, where the softmax scales them anyway. V: fp16 (u - 128) 2^(ev - e),
+//    exact down to 2^-24, with e the largest V exponent that the tile sees, found before the first block; O is multiplied by
+//    2^(e - 133) at the end. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
+//    same layout read as MN-major B.
+//  * P is fp16 (11 significant bits), V too; the row sum adds the rounded P.
+//  * the tile's rows need not be consecutive in memory, so Q is copied by the converter warps as well.
+//
+// 3300 cycles per block of the two tiles, as the dense kernel: the softmax's exponentials and the MMAs bound it, the
+// converters (310 instructions a lane and block) fit beside them.
+#include "rl_common.cuh"
+#include "rl_host.h"
+
+namespace rl {
+namespace kvprompt {
+
+using kv::BT;
+using kv::HD;
+using kvattn::Div;
+
+constexpr int BQ = 128;
+constexpr int ROWS = 2 * BQ;          // rows per CTA
+constexpr int BKV = 128;              // keys per block
+constexpr int kThreads = 384;
+constexpr int KS = 3, VS = 2;         // operand stages
+constexpr int RING = 8;               // blocks whose scales are kept
+constexpr int SUB = 128 * 128;        // 128 rows of 64 16-bit values
+constexpr int TILE = 2 * SUB;
+constexpr int kQ = 0, kK = 2 * TILE, kV = kK + KS * TILE, kBar = kV + VS * TILE;
+constexpr int kBytes = 1024 + kBar + 1024;
+static_assert(kBytes <= 232448, "shared memory");
+constexpr int kTmemCols = 512, kOCol = 256;
+constexpr float kTau = 8.0f;
+constexpr int kRegsLaunch = 168, kRegsLow = 80, kRegsHigh = 208;   // as rl_attn.cu's two-tile kernel
+static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split above the launch's total");
+constexpr int kConv = 3;              // converter warps: 0, 2 and 3 (1 issues the MMAs)
+
+struct Barriers {
+  uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_full, drain;
+  uint32_t tmem_base;
+  int abort;
+  int e_max;                          // largest V exponent of the tile's keys
+  int task[4];                        // sequence, head, tile (or -1)
+  int v_poison;                       // first position of the first V block with a NaN or an infinity
+  alignas(8) uint8_t flag[RING][8];              // per block of 16 keys: 1 = K with a NaN or an infinity, 2 = absent
+  alignas(16) float scale[RING][8];   // per block of 16 keys: what its raw scores are multiplied by
+};
+static_assert(sizeof(Barriers) <= 1024, "barrier block");
+
+struct Args {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  kv::Pool pool;
+  kv::Batch batch;
+  const int32_t* row_limit;
+  float scale_log2;
+  uint16_t* o;
+  int64_t ldo;
+  Div group, hkv;
+  int page_sh, vec;                   // vec: rows of o are 16-byte aligned
+};
+
+// B operand stored [k][64 n] with the 128-byte swizzle (MN-major): 64-column groups SUB bytes apart, 8-row groups 1024.
+__device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(SUB >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// kind::f16 with fp16 A and B, B MN-major, fp32 D.
+__host__ __device__ constexpr uint32_t idesc_f16_bmn(int M, int N) {
+  return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// 16 keys of a block: lane l holds rows l / 8 + 4 i, codes 16 (l % 8) .. + 15.
+struct Unit {
+  uint4 c[4];
+  uint32_t e;       // exponent byte | 0x100 when the page is absent
+};
+
+// Write a unit's 16 rows into an operand tile (rows r0 ..): 32 bytes of 16-bit values per 16 codes, as two 16-byte chunks
+// at swizzled positions. Lanes of the second 64 dims write their chunks in the other order, so that the eight lanes of a
+// phase (one row) hit eight different bank groups.
+template <bool kIsV>
+__device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u, uint32_t mul, uint32_t add, int lane) {
+  const int j = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + (lane >> 3) + 4 * i;
+    const uint32_t w[4] = {u.c[i].x, u.c[i].y, u.c[i].z, u.c[i].w};
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = __byte_perm(w[k], kIsV ? 0x64646464u : 0u, 0x4140), hi = __byte_perm(w[k], kIsV ? 0x64646464u : 0u, 0x4342);
+      v[2 * k] = kIsV ? fma_f16x2(lo, mul, add) : fma_bf16x2(lo, mul, add);
+      v[2 * k + 1] = kIsV ? fma_f16x2(hi, mul, add) : fma_bf16x2(hi, mul, add);
+    }
+    uint8_t* at = tile + (j >> 2) * SUB + row * 128;
+    const int c0 = 2 * (j & 3), flip = j >> 2, x = row & 7;
+    const uint4 a = make_uint4(v[0], v[1], v[2], v[3]), b = make_uint4(v[4], v[5], v[6], v[7]);
+    *reinterpret_cast<uint4*>(at + (((c0 + flip) ^ x) << 4)) = flip ? b : a;
+    *reinterpret_cast<uint4*>(at + (((c0 + 1 - flip) ^ x) << 4)) = flip ? a : b;
+  }
+}
+
+// One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys.
+__device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0, int lim, const float* scale,
+                                              uint2 flags, bool o_live, float& m_run, float& l_run, uint64_t* p_bar,
+                                              int lane) {
+  uint32_t s[BKV];
+#pragma unroll
+  for (int c = 0; c < BKV / 32; ++c) {
+    uint32_t (&sc)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]);
+    RL_TMEM_LD32(ta + 32 * c, sc);
+  }
+  tmem_ld_wait_regs(s);
+  if (key0 + BKV - 1 > lim) {
+#pragma unroll
+    for (int c = 0; c < BKV; ++c)
+      if (key0 + c > lim) s[c] = 0xFF800000u;  // -inf
+  }
+  if (flags.x | flags.y) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t f = (i < 4 ? flags.x : flags.y) >> (8 * (i & 3));
+      if (f & 2) {
+#pragma unroll
+        for (int c = 16 * i; c < 16 * i + 16; ++c) s[c] = 0xFF800000u;
+      }
+      if ((f & 1) && key0 + 16 * i <= lim) l_run = __uint_as_float(0x7FC00000u);
+    }
+  }
+  const float4 sa = *reinterpret_cast<const float4*>(scale), sb = *reinterpret_cast<const float4*>(scale + 4);
+  const float scl[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int c = 16 * i; c < 16 * i + 16; c += 4) {
+      a = attn::max3f(a, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+      b = attn::max3f(b, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+    }
+    mx = fmaxf(mx, fmaxf(a, b) * scl[i]);
+  }
+  const bool raise = mx > m_run + kTau;
+  float alpha = 1.0f;
+  if (raise) {
+    alpha = exp2f(m_run - mx);
+    l_run *= alpha;
+    m_run = mx;
+  }
+  const bool rescale = o_live && __any_sync(0xffffffffu, raise);
+  const bool none = m_run == -INFINITY;
+  const float2 nm2 = make_float2(-m_run, -m_run);
+  float2 acc[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh) {
+    uint32_t pk[32];
+    if (none) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) pk[c] = 0u;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const int i = 64 * hh + 2 * c;
+        const float2 sc2 = make_float2(scl[i >> 4], scl[i >> 4]);
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, nm2);
+        pk[c] = kvattn::pack_h2(attn::ex2_approx(x.x), attn::ex2_approx(x.y));
+        acc[c & 3] = __fadd2_rn(acc[c & 3], kvattn::unpack_h2(pk[c]));
+      }
+    }
+    RL_TMEM_ST32(ta + 32 * hh, pk);
+    if (hh == 0 && rescale) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        RL_TMEM_LD32(to + 32 * c, o);
+        tmem_ld_wait_regs(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        RL_TMEM_ST32(to + 32 * c, o);
+        tmem_st_wait_regs(o);
+      }
+    }
+    tmem_st_wait_regs(pk);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&p_bar[hh]);
+  }
+  const float2 a01 = __fadd2_rn(acc[0], acc[1]), a23 = __fadd2_rn(acc[2], acc[3]);
+  const float2 a = __fadd2_rn(a01, a23);
+  l_run += a.x + a.y;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + kBar);
+  volatile int* abort = &bars->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0) {
+    // the task of this CTA: sequences in order, each with kv_heads x ceil(rows / 256) tiles, the last tile first
+    int64_t before = 0;
+    int found = -1, at = 0;
+    for (int b0 = 0; b0 < a.batch.B && found < 0; b0 += 32) {
+      const int b = b0 + lane;
+      int64_t n = 0;
+      if (b < a.batch.B) {
+        const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
+        if (s.ok) n = (s.n * a.group.d + ROWS - 1) / ROWS * a.pool.hkv;
+        else if (blockIdx.x == 0) report(kErrBadArgument);
+      }
+      int64_t end = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, end, d);
+        if (lane >= d) end += v;
+      }
+      const bool mine = static_cast<int64_t>(blockIdx.x) - before < end;
+      const uint32_t hit = __ballot_sync(0xffffffffu, mine);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        found = b0 + l;
+        at = static_cast<int>(blockIdx.x - before - __shfl_sync(0xffffffffu, end - n, l));
+      }
+      before += __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (lane == 0) {
+      bars->task[0] = found;
+      if (found >= 0) {
+        const kv::Seq s = kv::load_seq(a.batch, found, a.pool.page);
+        const int tiles = static_cast<int>((s.n * a.group.d + ROWS - 1) / ROWS);
+        const uint32_t t = static_cast<uint32_t>(at) / a.hkv;
+        bars->task[1] = at - static_cast<int>(t) * a.pool.hkv;
+        bars->task[2] = tiles - 1 - static_cast<int>(t);
+      }
+      mbar_init(&bars->q_full, kConv);
+      for (int i = 0; i < KS; ++i) mbar_init(&bars->k_full[i], kConv), mbar_init(&bars->k_empty[i], 1);
+      for (int i = 0; i < VS; ++i) mbar_init(&bars->v_full[i], kConv), mbar_init(&bars->v_empty[i], 1);
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&bars->s_full[t], 1);
+        mbar_init(&bars->p_full[t][0], 4);
+        mbar_init(&bars->p_full[t][1], 4);
+      }
+      mbar_init(&bars->o_full, 1);
+      mbar_init(&bars->drain, 1);
+      bars->abort = 0;
+      bars->e_max = 0;
+      bars->v_poison = INT32_MAX;
+      fence_mbar_init();
+    }
+  }
+  __syncthreads();
+  const int b = bars->task[0];
+  if (b < 0) return;   // (the grid is an upper bound)
+  if (warp == 0) {
+    tmem_alloc(&bars->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const int h = bars->task[1];
+  const uint32_t row0 = static_cast<uint32_t>(bars->task[2]) * ROWS;
+  const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
+  const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;
+  // the keys that any row sees: limits grow along the rows, unless row_limit gives them
+  const uint32_t last_row = min(row0 + ROWS, rows) - 1;
+  const int64_t kmax = a.row_limit ? s.len : s.len - s.n + last_row / a.group + 1;
+  const int nblk = static_cast<int>((kmax + BKV - 1) / BKV);      // >= 1
+
+  if (warp < 4) {
+    attn::setmaxnreg_dec<kRegsLow>();
+    if (warp != 1) {
+      // ---------------- converters ----------------
+      const int cw = warp == 0 ? 0 : warp - 1;
+      auto block_at = [&](int u) -> int {       // pool index of the sequence's 16-key block u; -1 beyond the keys, -2 absent
+        const int64_t pos = static_cast<int64_t>(u) * BT;
+        if (pos >= kmax) return -1;
+        const int pg = __ldg(a.batch.table + b * a.batch.ld + (pos >> a.page_sh));
+        if (static_cast<uint32_t>(pg) >= a.pool.pages) return -2;
+        return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + ((static_cast<int>(pos) & (a.pool.page - 1)) >> 4);
+      };
+      // the largest V exponent
+      int e = 0;
+      const int units = static_cast<int>((kmax + BT - 1) / BT);
+#pragma unroll 4
+      for (int u = cw * 32 + lane; u < units; u += kConv * 32) {
+        const int blk = block_at(u);
+        if (blk == -2) report(kErrBadArgument);
+        const int ve = blk >= 0 ? a.pool.ve[blk] : 0;
+        if (ve != 255) e = max(e, ve);
+        else atomicMin(&bars->v_poison, u * BT);
+      }
+      e = __reduce_max_sync(0xffffffffu, e);
+      if (lane == 0) atomicMax(&bars->e_max, e);
+      // Q: 256 rows x 16 chunks of 16 bytes
+      for (int i = cw * 32 + lane; i < ROWS * 16; i += kConv * 32) {
+        const int r = i >> 4, c = i & 15;
+        const uint32_t rr = row0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (rr < rows) {
+          const uint32_t j = rr / a.group;
+          v = *reinterpret_cast<const uint4*>(a.q + (s.s0 + j) * a.q_st + (h * a.group.d + rr - j * a.group.d) * a.q_sh + 8 * c);
+        }
+        const int x = r & 127;
+        *reinterpret_cast<uint4*>(smem + kQ + (r >> 7) * TILE + (c >> 3) * SUB + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full);
+      asm volatile("bar.sync 1, 96;" ::: "memory");               // the converters' maxima are joined
+      const int em = bars->e_max;
+
+      // items K(0), V(0), K(1), V(1), ..; warp cw takes units cw, cw + 3, cw + 6 of an item's eight. The codes of an item
+      // are loaded while the one before is converted, its page lookups one item earlier still.
+      Unit u[3];
+      int idx[3];
+      const int items = 2 * nblk;
+      auto lookup = [&](int it) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) idx[i] = it < items && cw + 3 * i < 8 ? block_at((it >> 1) * 8 + cw + 3 * i) : -1;
+      };
+      auto load = [&](int it) {
+        const uint8_t* codes = it & 1 ? a.pool.v : a.pool.k;
+        const uint8_t* exps = it & 1 ? a.pool.ve : a.pool.ke;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          u[i].e = idx[i] == -2 ? 0x100u : 0u;
+          if (idx[i] >= 0) {
+            const uint8_t* p = codes + static_cast<int64_t>(idx[i]) * (BT * HD) + lane * 16;
+            u[i].e = exps[idx[i]];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[i].c[k] = *reinterpret_cast<const uint4*>(p + k * 512);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[i].c[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+          }
+        }
+      };
+      lookup(0);
+      load(0);
+      lookup(1);
+      for (int it = 0; it < items; ++it) {
+        const int j = it >> 1, is_v = it & 1;
+        const int st = is_v ? j % VS : j % KS;
+        const uint32_t ph = is_v ? (j / VS) & 1 : (j / KS) & 1;
+        uint64_t* empty = is_v ? &bars->v_empty[st] : &bars->k_empty[st];
+        uint64_t* full = is_v ? &bars->v_full[st] : &bars->k_full[st];
+        if (!mbar_wait_warp(empty, ph ^ 1, abort)) break;
+        uint8_t* tile = smem + (is_v ? kV : kK) + st * TILE;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const int k = cw + 3 * i;
+          if (k < 8) {
+            if (is_v) {
+              const int d = em - static_cast<int>(u[i].e & 255u);
+              // 2^-d and -1152 2^-d in fp16; a poisoned block's codes count as they are (its rows become NaN), scale 1
+              const float f = d < 0 ? 1.0f : d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
+              write_unit<true>(tile, 16 * k, u[i], kvattn::pack_h2(f, f), kvattn::pack_h2(-1152.0f * f, -1152.0f * f), lane);
+            } else {
+              write_unit<false>(tile, 16 * k, u[i], 0x7F007F00u, 0xC000C000u, lane);
+              if (lane == 0) {                                    // (the last use of this slot was eight blocks ago)
+                const bool poisoned = u[i].e == 255u;
+                bars->scale[j % RING][k] = poisoned ? 1.0f : bfp16_scale(u[i].e & 255u) * 64.0f * a.scale_log2;
+                bars->flag[j % RING][k] = static_cast<uint8_t>((poisoned ? 1 : 0) | (u[i].e & 0x100u ? 2 : 0));
+              }
+            }
+          }
+        }
+        if (it + 1 < items) {
+          load(it + 1);
+          lookup(it + 2);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+      }
+    } else {
+      // ---------------- MMA issuer (warp-wide, elected lane issues) ----------------
+      constexpr uint32_t idesc_s = idesc_bf16(BQ, BKV);
+      constexpr uint32_t idesc_o = idesc_f16_bmn(BQ, HD);
+      bool any = false;
+      const uint32_t qa0 = smem_u32(smem + kQ);
+      auto qk = [&](int t, int j) -> bool {
+        const int st = j % KS;
+        if (!mbar_wait_warp(&bars->k_full[st], (j / KS) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t qa = qa0 + t * TILE, kb = smem_u32(smem + kK + st * TILE);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint64_t adesc = sdesc_kmajor_sw128(qa + (k >> 2) * SUB) + 2 * (k & 3);
+            const uint64_t bdesc = sdesc_kmajor_sw128(kb + (k >> 2) * SUB) + 2 * (k & 3);
+            umma_ss(tmem + t * BKV, adesc, bdesc, idesc_s, k ? 1u : 0u);
+          }
+          umma_commit(&bars->s_full[t]);
+          if (t == 1) umma_commit(&bars->k_empty[st]);
+        }
+        __syncwarp();
+        any = true;
+        return true;
+      };
+      auto pv = [&](int t, int j) -> bool {
+        const int st = j % VS;
+        if (!mbar_wait_warp(&bars->v_full[st], (j / VS) & 1, abort)) return false;
+        const uint32_t vb = smem_u32(smem + kV + st * TILE);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (!mbar_wait_warp(&bars->p_full[t][hh], j & 1, abort)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 4 * hh; k < 4 * hh + 4; ++k)
+              umma_ts(tmem + kOCol + t * HD, tmem + t * BKV + k * 8, sdesc_mnmajor_sw128(vb + k * 2048), idesc_o,
+                      (j | k) ? 1u : 0u);
+            if (hh == 1 && t == 1) umma_commit(&bars->v_empty[st]);
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      bool ok = mbar_wait_warp(&bars->q_full, 0, abort) && qk(0, 0) && qk(1, 0);
+      for (int j = 1; ok && j < nblk; ++j) ok = pv(0, j - 1) && qk(0, j) && pv(1, j - 1) && qk(1, j);
+      if (ok) ok = pv(0, nblk - 1) && pv(1, nblk - 1);
+      if (elect_one()) {
+        if (ok) umma_commit(&bars->o_full);
+        if (!ok && any) {
+          umma_commit(&bars->drain);
+          mbar_drain(&bars->drain, 0);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    attn::setmaxnreg_inc<kRegsHigh>();
+    // ---------------- softmax of tile t (thread = row = TMEM lane) ----------------
+    const int t = (warp - 4) >> 2, q = warp & 3;
+    const uint32_t row = row0 + t * BQ + 32 * q + lane;
+    const uint32_t lane_off = (32u * q) << 16;
+    const uint32_t ta = tmem + t * BKV + lane_off, to = tmem + kOCol + t * HD + lane_off;
+    const uint32_t jr = row / a.group;
+    int lim = -1;
+    if (row < rows) {
+      lim = static_cast<int>(s.len - s.n + jr);
+      if (a.row_limit) lim = min(static_cast<int>(s.len) - 1, __ldg(a.row_limit + s.s0 + jr));
+    }
+    float m_run = -INFINITY, l_run = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < nblk; ++j) {
+      if (!mbar_wait(&bars->s_full[t], j & 1, abort)) { ok = false; break; }
+      tc_fence_after();
+      softmax_block(ta, to, j * BKV, lim, bars->scale[j % RING], *reinterpret_cast<const uint2*>(bars->flag[j % RING]), j > 0,
+                    m_run, l_run, bars->p_full[t], lane);
+    }
+    if (ok && mbar_wait(&bars->o_full, 0, abort)) {
+      tc_fence_after();
+      if (bars->v_poison <= lim) l_run = __uint_as_float(0x7FC00000u);
+      const float inv = l_run == 0.0f ? 0.0f : bfp16_scale(static_cast<uint32_t>(bars->e_max)) / l_run;
+      uint16_t* orow = a.o + (s.s0 + jr) * a.ldo + (h * a.group.d + row - jr * a.group.d) * HD;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        RL_TMEM_LD32(to + 32 * c, o);
+        tmem_ld_wait_regs(o);
+        if (row < rows) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = attn::pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          if (a.vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(orow + 32 * c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              orow[32 * c + 2 * i] = static_cast<uint16_t>(w[i]);
+              orow[32 * c + 2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// The register split waits for registers that the launch must have brought (see rl_attn.cu): checked once per device.
+inline int launch(int64_t tasks, const Args& a, cudaStream_t stream) {
+  static int regs = 0;
+  if (regs == 0) {
+    cudaFuncAttributes fa;
+    RL_TRY_CUDA(cudaFuncGetAttributes(&fa, prompt_kernel));
+    regs = fa.numRegs;
+  }
+  RL_REQUIRE(regs == kRegsLaunch, RL_ERR_UNSUPPORTED, "rl_kv_attention: compiled with %d registers a thread, its register "
+             "split needs %d", regs, kRegsLaunch);
+  RL_TRY_CUDA(cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  prompt_kernel<<<static_cast<unsigned>(tasks), kThreads, kBytes, stream>>>(a);
+  RL_TRY_CUDA(cudaGetLastError());
+  return RL_OK;
+}
+
+}  // namespace kvprompt
+}  // namespace rl

@@ -541,5 +541,11 @@ def set_attention_variant(v):
     return L.lib().rl_set_attention_variant(int(v))
 
 
+def set_kv_attention_path(v):
+    """0 = by shape (default), 1 = the kernel that splits keys over the GPU, 2 = the tcgen05 prompt kernel; returns the
+    previous choice."""
+    return L.lib().rl_set_kv_attention_path(int(v))
+
+
 def device_status():
     return L.device_status()

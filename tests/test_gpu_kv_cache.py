@@ -21,6 +21,15 @@ def env():
     return torch, ops, _lib, torch.device("cuda:0")
 
 
+@pytest.fixture(params=["split", "prompt"])
+def path(request, env):
+    """Both kernels of kv_attention take every shape."""
+    ops = env[1]
+    before = ops.set_kv_attention_path({"split": 1, "prompt": 2}[request.param])
+    yield request.param
+    ops.set_kv_attention_path(before)
+
+
 def bf16(torch, a, dev):
     return torch.from_numpy(O.bf16_bits(np.asarray(a, np.float32)).view(np.int16)).to(dev).view(torch.bfloat16)
 
@@ -189,11 +198,12 @@ ATTENDS = [  # kv lengths, new tokens, heads, K/V heads, page
     ([70, 5, 200], [4, 5, 1], 4, 2, 16), ([50, 64, 90], [0, 3, 0], 4, 1, 16), ([130], [130], 4, 2, 32),
     ([257, 40], [100, 40], 8, 2, 16), ([90, 33], [60, 33], 12, 1, 256), ([2500], [3], 16, 1, 64),
     ([40 + 13 * i for i in range(50)], [1 + i % 3 for i in range(50)], 4, 2, 16),
+    ([400, 130, 700], [300, 130, 129], 6, 2, 64), ([128, 256, 129], [64, 64, 65], 4, 1, 32),
 ]
 
 
 @pytest.mark.parametrize("kv,new,H,hkv,page", ATTENDS)
-def test_attention(env, kv, new, H, hkv, page):
+def test_attention(env, path, kv, new, H, hkv, page):
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, kv, new, hkv, page, layers=2, layer=1, seed=sum(kv) + H, wide=len(kv) % 3)
     q = O.bf16_round((c.rng.standard_normal((c.T, H, 128)) * 2).astype(np.float32))
@@ -206,7 +216,7 @@ def test_attention(env, kv, new, H, hkv, page):
     assert torch.equal(again, got)
 
 
-def test_attention_sharp_and_wide_scores(env):
+def test_attention_sharp_and_wide_scores(env, path):
     """Large logits (one key dominates, the maximum rises along the sequence) and rows of very different magnitude."""
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, [400, 90], [2, 9], 2, 32, seed=5)
@@ -217,7 +227,7 @@ def test_attention_sharp_and_wide_scores(env):
     check_attention(got, *c.oracle(q))
 
 
-def test_attention_blocks_of_very_different_scale(env):
+def test_attention_blocks_of_very_different_scale(env, path):
     """V and K blocks from 2^-40 to 2^40 and all-zero ones, in every order."""
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, [700, 300], [1, 3], 2, 16, seed=15)
@@ -235,7 +245,7 @@ def test_attention_blocks_of_very_different_scale(env):
     check_attention(got, *c.oracle(q))
 
 
-def test_attention_row_limits(env):
+def test_attention_row_limits(env, path):
     """Per-row limits: none visible (zeros), one key, past the end, and beyond the causal limit."""
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, [100, 37], [6, 5], 2, 16, seed=6)
@@ -247,7 +257,7 @@ def test_attention_row_limits(env):
     assert (got[0] == 0).all() and (got[6] == 0).all()
 
 
-def test_attention_strides_scale(env):
+def test_attention_strides_scale(env, path):
     """q (H, T, 128) as qkv_post leaves it, and a caller's scale."""
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, [77], [9], 1, 64, seed=8)
@@ -258,7 +268,7 @@ def test_attention_strides_scale(env):
     check_attention(got, *c.oracle(q * np.float32(0.25)))
 
 
-def test_attention_poisoned_block(env):
+def test_attention_poisoned_block(env, path):
     """A block that took in a NaN gives NaN to the rows that see it and to no other."""
     torch, ops, L, dev = env
     for which in ("k", "v"):
@@ -272,7 +282,7 @@ def test_attention_poisoned_block(env):
         assert np.abs(got[:8] - clean[:8].reshape(8, -1)).max() < 0.1
 
 
-def test_bad_pages_and_sequences_are_reported(env):
+def test_bad_pages_and_sequences_are_reported(env, path):
     """A page outside the pool: its keys count as absent. Impossible sequences are left out. Both set the error word."""
     torch, ops, L, dev = env
     c = Case(torch, ops, dev, [100, 40], [2, 1], 2, 16, seed=10)
@@ -326,7 +336,7 @@ def test_copy_pages(env, n, layers, hkv, page):
         assert torch.equal(got, w)
 
 
-def test_append_and_attend_in_a_graph(env):
+def test_append_and_attend_in_a_graph(env, path):
     """A captured decode step follows the device-side lengths when it is replayed."""
     torch, ops, L, dev = env
     H, hkv = 4, 2
