@@ -4,7 +4,7 @@
 // With K = 2^(ek-133) mk per block of 16 tokens, s is an fp16 product q~ . mk (mk is an integer in [-128, 127], exact;
 // q~ is q times a power of two per row that puts the row's largest value in [2^14, 2^15), exact for every value within
 // 2^-28 of it) times one fp32 factor per block and row. P is rounded to fp16 (11 significant bits, half a step 2^-11
-// of each weight; the row sum adds the rounded weights) and P . mv of a block, again with exact integers, is scaled by
+// of each weight; the row sum adds them unrounded) and P . mv of a block, again with exact integers, is scaled by
 // 2^(ev-133) as it is added to the fp32 accumulator. So the only roundings are P's and fp32's.
 //
 // The rows of one K/V head that share its keys (tokens of a sequence x query heads of the group) are the N side of
@@ -84,11 +84,6 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float2 unpack_h2(uint32_t h) {
-  float2 f;
-  asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;}" : "=f"(f.x), "=f"(f.y) : "r"(h));
-  return f;
-}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -166,19 +161,18 @@ struct Acc {
   int er;                // O is in units of 2^(er - 133)
 };
 
-// P^T of a block times 2^shift, in the B layout; the row sums add the rounded weights times `unit`.
+// P^T of a block times 2^shift, in the B layout; the row sums add the weights, before their rounding, times `unit`.
 template <int NT>
 __device__ __forceinline__ void weights(const float (&s)[NT][4], Acc<NT>& acc, float shift, float unit, uint32_t (&p)[NT][2]) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float m0 = acc.m[nt][0] - shift, m1 = acc.m[nt][1] - shift;
-    const uint32_t lo = pack_h2(exp2_approx(s[nt][0] - m0), exp2_approx(s[nt][1] - m1));
-    const uint32_t hi = pack_h2(exp2_approx(s[nt][2] - m0), exp2_approx(s[nt][3] - m1));
-    const float2 f = unpack_h2(lo), h = unpack_h2(hi);
-    acc.l[nt][0] = fmaf(unit, f.x + h.x, acc.l[nt][0]);
-    acc.l[nt][1] = fmaf(unit, f.y + h.y, acc.l[nt][1]);
-    p[nt][0] = movmatrix(lo);
-    p[nt][1] = movmatrix(hi);
+    const float e0 = exp2_approx(s[nt][0] - m0), e1 = exp2_approx(s[nt][1] - m1);
+    const float e2 = exp2_approx(s[nt][2] - m0), e3 = exp2_approx(s[nt][3] - m1);
+    acc.l[nt][0] = fmaf(unit, e0 + e2, acc.l[nt][0]);
+    acc.l[nt][1] = fmaf(unit, e1 + e3, acc.l[nt][1]);
+    p[nt][0] = movmatrix(pack_h2(e0, e1));
+    p[nt][1] = movmatrix(pack_h2(e2, e3));
   }
 }
 

@@ -11,7 +11,7 @@
 //    exact down to 2^-24, with e the largest V exponent that the tile sees, found before the first block; O is multiplied by
 //    2^(e - 133) at the end. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
 //    same layout read as MN-major B.
-//  * P is fp16 (11 significant bits), V too; the row sum adds the rounded P.
+//  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
 //  * the tile's rows need not be consecutive in memory, so Q is copied by the converter warps as well.
 //
 // 3300 cycles per block of the two tiles, as the dense kernel: the softmax's exponentials and the MMAs bound it, the
@@ -30,11 +30,12 @@ constexpr int BQ = 128;
 constexpr int ROWS = 2 * BQ;          // rows per CTA
 constexpr int BKV = 128;              // keys per block
 constexpr int kThreads = 384;
-constexpr int KS = 3, VS = 2;         // operand stages
+constexpr int KS = 2, VS = 2;         // operand stages
 constexpr int RING = 8;               // blocks whose scales are kept
 constexpr int SUB = 128 * 128;        // 128 rows of 64 16-bit values
 constexpr int TILE = 2 * SUB;
-constexpr int kQ = 0, kK = 2 * TILE, kV = kK + KS * TILE, kBar = kV + VS * TILE;
+constexpr int RAW = BKV * HD;         // a block's codes of K or of V
+constexpr int kQ = 0, kK = 2 * TILE, kV = kK + KS * TILE, kRaw = kV + VS * TILE, kBar = kRaw + 2 * RAW;
 constexpr int kBytes = 1024 + kBar + 1024;
 static_assert(kBytes <= 232448, "shared memory");
 constexpr int kTmemCols = 512, kOCol = 256;
@@ -94,22 +95,17 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
   return d;
 }
 
-// 16 keys of a block: lane l holds rows l / 8 + 4 i, codes 16 (l % 8) .. + 15.
-struct Unit {
-  uint4 c[4];
-  uint32_t e;       // exponent byte | 0x100 when the page is absent
-};
-
-// Write a unit's 16 rows into an operand tile (rows r0 ..): 32 bytes of 16-bit values per 16 codes, as two 16-byte chunks
-// at swizzled positions. Lanes of the second 64 dims write their chunks in the other order, so that the eight lanes of a
-// phase (one row) hit eight different bank groups.
+// Turn a unit (16 keys) into 16 rows of an operand tile (rows r0 ..): 32 bytes of 16-bit values per 16 codes, as two
+// 16-byte chunks at swizzled positions. Step i of a lane is row l / 4 + 8 (i / 2), codes 16 (l % 4) + 64 (i % 2) ..: the
+// eight lanes of a shared-memory phase then write an even and an odd row, whose chunks lie in eight different bank groups.
+__device__ __forceinline__ int unit_row(int i, int lane) { return (lane >> 2) + 8 * (i >> 1); }
+__device__ __forceinline__ int unit_code(int i, int lane) { return 16 * (lane & 3) + 64 * (i & 1); }
 template <bool kIsV>
-__device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u, uint32_t mul, uint32_t add, int lane) {
-  const int j = lane & 7;
+__device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const uint8_t* raw, uint32_t mul, uint32_t add, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = r0 + (lane >> 3) + 4 * i;
-    const uint32_t w[4] = {u.c[i].x, u.c[i].y, u.c[i].z, u.c[i].w};
+    const uint4 u = *reinterpret_cast<const uint4*>(raw + 512 * i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     uint32_t v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -117,11 +113,10 @@ __device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u,
       v[2 * k] = kIsV ? fma_f16x2(lo, mul, add) : fma_bf16x2(lo, mul, add);
       v[2 * k + 1] = kIsV ? fma_f16x2(hi, mul, add) : fma_bf16x2(hi, mul, add);
     }
-    uint8_t* at = tile + (j >> 2) * SUB + row * 128;
-    const int c0 = 2 * (j & 3), flip = j >> 2, x = row & 7;
-    const uint4 a = make_uint4(v[0], v[1], v[2], v[3]), b = make_uint4(v[4], v[5], v[6], v[7]);
-    *reinterpret_cast<uint4*>(at + (((c0 + flip) ^ x) << 4)) = flip ? b : a;
-    *reinterpret_cast<uint4*>(at + (((c0 + 1 - flip) ^ x) << 4)) = flip ? a : b;
+    uint8_t* at = tile + (i & 1) * SUB + (r0 + unit_row(i, lane)) * 128;
+    const int c0 = 2 * (lane & 3), x = (lane >> 2) & 7;             // r0 and 8 (i / 2) are multiples of 8
+    *reinterpret_cast<uint4*>(at + ((c0 ^ x) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<uint4*>(at + (((c0 + 1) ^ x) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
   }
 }
 
@@ -188,8 +183,9 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
         const int i = 64 * hh + 2 * c;
         const float2 sc2 = make_float2(scl[i >> 4], scl[i >> 4]);
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, nm2);
-        pk[c] = kvattn::pack_h2(attn::ex2_approx(x.x), attn::ex2_approx(x.y));
-        acc[c & 3] = __fadd2_rn(acc[c & 3], kvattn::unpack_h2(pk[c]));
+        const float2 e = make_float2(attn::ex2_approx(x.x), attn::ex2_approx(x.y));
+        pk[c] = kvattn::pack_h2(e.x, e.y);
+        acc[c & 3] = __fadd2_rn(acc[c & 3], e);
       }
     }
     RL_TMEM_ST32(ta + 32 * hh, pk);
@@ -337,70 +333,77 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       asm volatile("bar.sync 1, 96;" ::: "memory");               // the converters' maxima are joined
       const int em = bars->e_max;
 
-      // items K(0), V(0), K(1), V(1), ..; warp cw takes units cw, cw + 3, cw + 6 of an item's eight. The codes of an item
-      // are loaded while the one before is converted, its page lookups one item earlier still.
-      Unit u[3];
+      // Warp cw converts units cw, cw + 3 and cw + 6 of each block's eight. The codes of block j + 1 are copied into the
+      // raw buffer as soon as block j's have been read (each lane reads what it copied itself), so a copy has the time
+      // of a whole block; page lookups run one block further ahead.
+      uint8_t* raw = smem + kRaw + lane * 16;
       int idx[3];
-      const int items = 2 * nblk;
-      auto lookup = [&](int it) {
+      uint32_t ke[3], ve[3];                                      // exponents of the block in the raw buffer | 0x100 absent
+      auto lookup = [&](int j) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) idx[i] = it < items && cw + 3 * i < 8 ? block_at((it >> 1) * 8 + cw + 3 * i) : -1;
+        for (int i = 0; i < 3; ++i) idx[i] = j < nblk && cw + 3 * i < 8 ? block_at(j * 8 + cw + 3 * i) : -1;
       };
-      auto load = [&](int it) {
-        const uint8_t* codes = it & 1 ? a.pool.v : a.pool.k;
-        const uint8_t* exps = it & 1 ? a.pool.ve : a.pool.ke;
+      auto copy = [&](int v, uint32_t (&e)[3]) {
+        const uint8_t* codes = v ? a.pool.v : a.pool.k;
+        const uint8_t* exps = v ? a.pool.ve : a.pool.ke;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          u[i].e = idx[i] == -2 ? 0x100u : 0u;
-          if (idx[i] >= 0) {
-            const uint8_t* p = codes + static_cast<int64_t>(idx[i]) * (BT * HD) + lane * 16;
-            u[i].e = exps[idx[i]];
+          const int64_t blk = max(idx[i], 0);                     // beyond the keys, or absent: any block, with weight zero
+          e[i] = (idx[i] < 0 ? 0u : exps[blk]) | (idx[i] == -2 ? 0x100u : 0u);
+          if (cw + 3 * i < 8) {
+            const uint8_t* p = codes + blk * (BT * HD);
+            const uint32_t d = smem_u32(raw) + v * RAW + (cw + 3 * i) * (BT * HD);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) u[i].c[k] = *reinterpret_cast<const uint4*>(p + k * 512);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) u[i].c[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            for (int k = 0; k < 4; ++k) kvattn::cp_async16(d + 512 * k, p + unit_row(k, lane) * HD + unit_code(k, lane));
           }
         }
+        kvattn::cp_commit();
       };
       lookup(0);
-      load(0);
+      copy(0, ke);
+      copy(1, ve);
       lookup(1);
-      for (int it = 0; it < items; ++it) {
-        const int j = it >> 1, is_v = it & 1;
-        const int st = is_v ? j % VS : j % KS;
-        const uint32_t ph = is_v ? (j / VS) & 1 : (j / KS) & 1;
-        uint64_t* empty = is_v ? &bars->v_empty[st] : &bars->k_empty[st];
-        uint64_t* full = is_v ? &bars->v_full[st] : &bars->k_full[st];
-        if (!mbar_wait_warp(empty, ph ^ 1, abort)) break;
-        uint8_t* tile = smem + (is_v ? kV : kK) + st * TILE;
+      for (int j = 0; j < nblk; ++j) {
+        const int ks = j % KS, vs = j % VS;
+        if (!mbar_wait_warp(&bars->k_empty[ks], ((j / KS) & 1) ^ 1, abort)) break;
+        kvattn::cp_wait<1>();
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
           const int k = cw + 3 * i;
           if (k < 8) {
-            if (is_v) {
-              const int d = em - static_cast<int>(u[i].e & 255u);
-              // 2^-d and -1152 2^-d in fp16; a poisoned block's codes count as they are (its rows become NaN), scale 1
-              const float f = d < 0 ? 1.0f : d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
-              write_unit<true>(tile, 16 * k, u[i], kvattn::pack_h2(f, f), kvattn::pack_h2(-1152.0f * f, -1152.0f * f), lane);
-            } else {
-              write_unit<false>(tile, 16 * k, u[i], 0x7F007F00u, 0xC000C000u, lane);
-              if (lane == 0) {                                    // (the last use of this slot was eight blocks ago)
-                const bool poisoned = u[i].e == 255u;
-                bars->scale[j % RING][k] = poisoned ? 1.0f : bfp16_scale(u[i].e & 255u) * 64.0f * a.scale_log2;
-                bars->flag[j % RING][k] = static_cast<uint8_t>((poisoned ? 1 : 0) | (u[i].e & 0x100u ? 2 : 0));
-              }
+            write_unit<false>(smem + kK + ks * TILE, 16 * k, raw + k * (BT * HD), 0x7F007F00u, 0xC000C000u, lane);
+            if (lane == 0) {                                      // (the last use of this slot was eight blocks ago)
+              const bool poisoned = ke[i] == 255u;
+              bars->scale[j % RING][k] = poisoned ? 1.0f : bfp16_scale(ke[i] & 255u) * 64.0f * a.scale_log2;
+              bars->flag[j % RING][k] = static_cast<uint8_t>((poisoned ? 1 : 0) | (ke[i] & 0x100u ? 2 : 0));
             }
           }
         }
-        if (it + 1 < items) {
-          load(it + 1);
-          lookup(it + 2);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->k_full[ks]);
+        copy(0, ke);
+        if (!mbar_wait_warp(&bars->v_empty[vs], ((j / VS) & 1) ^ 1, abort)) break;
+        kvattn::cp_wait<1>();
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const int k = cw + 3 * i;
+          if (k < 8) {
+            // 2^-d and -1152 2^-d in fp16. Keys beyond the end or absent have exponent 0: d > 24 unless all are near 0,
+            // and P = 0 in any case; a poisoned block's codes count as they are (the rows that see it become NaN).
+            const int d = em - static_cast<int>(ve[i] & 255u);
+            const float f = d < 0 ? 1.0f : d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
+            write_unit<true>(smem + kV + vs * TILE, 16 * k, raw + RAW + k * (BT * HD), kvattn::pack_h2(f, f),
+                             kvattn::pack_h2(-1152.0f * f, -1152.0f * f), lane);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(full);
+        if (lane == 0) mbar_arrive(&bars->v_full[vs]);
+        copy(1, ve);
+        lookup(j + 2);
       }
+      kvattn::cp_wait<0>();
     } else {
       // ---------------- MMA issuer (warp-wide, elected lane issues) ----------------
       constexpr uint32_t idesc_s = idesc_bf16(BQ, BKV);
