@@ -30,18 +30,15 @@ constexpr int BQ = 128;
 constexpr int ROWS = 2 * BQ;          // rows per CTA
 constexpr int BKV = 128;              // keys per block
 constexpr int kThreads = 384;
-constexpr int KS = 2, VS = 2;         // operand stages
+constexpr int KS = 3, VS = 2;         // operand stages
 constexpr int RING = 8;               // blocks whose scales are kept
 constexpr int SUB = 128 * 128;        // 128 rows of 64 16-bit values
 constexpr int TILE = 2 * SUB;
-constexpr int RAW = BKV * HD;         // a block's codes of K or of V
-constexpr int kQ = 0, kK = 2 * TILE, kV = kK + KS * TILE, kRaw = kV + VS * TILE, kBar = kRaw + 2 * RAW;
+constexpr int kQ = 0, kK = 2 * TILE, kV = kK + KS * TILE, kBar = kV + VS * TILE;
 constexpr int kBytes = 1024 + kBar + 1024;
 static_assert(kBytes <= 232448, "shared memory");
 constexpr int kTmemCols = 512, kOCol = 256;
 constexpr float kTau = 8.0f;
-constexpr int kRegsLaunch = 168, kRegsLow = 80, kRegsHigh = 208;   // as rl_attn.cu's two-tile kernel
-static_assert(128 * kRegsLow + 256 * kRegsHigh <= kThreads * kRegsLaunch, "register split above the launch's total");
 constexpr int kConv = 3;              // converter warps: 0, 2 and 3 (1 issues the MMAs)
 
 struct Barriers {
@@ -95,17 +92,22 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
   return d;
 }
 
-// Turn a unit (16 keys) into 16 rows of an operand tile (rows r0 ..): 32 bytes of 16-bit values per 16 codes, as two
+// 16 keys of a block in the lane's registers, with the block's exponent byte (0x100: absent or beyond the keys).
+struct Unit {
+  uint4 c[4];
+  uint32_t e;
+};
+
+// Turn a unit into 16 rows of an operand tile (rows r0 ..): 32 bytes of 16-bit values per 16 codes, as two
 // 16-byte chunks at swizzled positions. Step i of a lane is row l / 4 + 8 (i / 2), codes 16 (l % 4) + 64 (i % 2) ..: the
 // eight lanes of a shared-memory phase then write an even and an odd row, whose chunks lie in eight different bank groups.
 __device__ __forceinline__ int unit_row(int i, int lane) { return (lane >> 2) + 8 * (i >> 1); }
 __device__ __forceinline__ int unit_code(int i, int lane) { return 16 * (lane & 3) + 64 * (i & 1); }
 template <bool kIsV>
-__device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const uint8_t* raw, uint32_t mul, uint32_t add, int lane) {
+__device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u, uint32_t mul, uint32_t add, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 u = *reinterpret_cast<const uint4*>(raw + 512 * i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {u.c[i].x, u.c[i].y, u.c[i].z, u.c[i].w};
     uint32_t v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -120,30 +122,32 @@ __device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const uint8_t*
   }
 }
 
-// One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys.
+// What hides a score of the 32 columns from `c0`: keys beyond the row's limit, and blocks of absent pages.
+__device__ __forceinline__ void mask32(uint32_t (&s)[32], int key, int lim, uint32_t absent) {
+  if (key + 31 > lim) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (key + c > lim) s[c] = 0xFF800000u;  // -inf
+  }
+  if (absent) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (absent >> (c >> 4) & 1) s[c] = 0xFF800000u;
+  }
+}
+
+// One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys. S
+// is read from TMEM twice, 32 columns at a time, for the maximum and for the exponentials: holding the row would take 128
+// registers of every softmax thread. P of columns c .. is written to the first half of columns that were read before.
 __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0, int lim, const float* scale,
                                               uint2 flags, bool o_live, float& m_run, float& l_run, uint64_t* p_bar,
                                               int lane) {
-  uint32_t s[BKV];
-#pragma unroll
-  for (int c = 0; c < BKV / 32; ++c) {
-    uint32_t (&sc)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]);
-    RL_TMEM_LD32(ta + 32 * c, sc);
-  }
-  tmem_ld_wait_regs(s);
-  if (key0 + BKV - 1 > lim) {
-#pragma unroll
-    for (int c = 0; c < BKV; ++c)
-      if (key0 + c > lim) s[c] = 0xFF800000u;  // -inf
-  }
+  uint32_t absent = 0;   // bit i: 16-key block i
   if (flags.x | flags.y) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t f = (i < 4 ? flags.x : flags.y) >> (8 * (i & 3));
-      if (f & 2) {
-#pragma unroll
-        for (int c = 16 * i; c < 16 * i + 16; ++c) s[c] = 0xFF800000u;
-      }
+      absent |= (f >> 1 & 1) << i;
       if ((f & 1) && key0 + 16 * i <= lim) l_run = __uint_as_float(0x7FC00000u);
     }
   }
@@ -151,14 +155,26 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
   const float scl[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
   float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float a = -INFINITY, b = -INFINITY;
+  for (int h = 0; h < 2; ++h) {
+    uint32_t s[2][32];
+    RL_TMEM_LD32(ta + 64 * h, s[0]);
+    RL_TMEM_LD32(ta + 64 * h + 32, s[1]);
+    tmem_ld_wait_regs(s[0]);
+    tmem_ld_wait_regs(s[1]);
 #pragma unroll
-    for (int c = 16 * i; c < 16 * i + 16; c += 4) {
-      a = attn::max3f(a, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-      b = attn::max3f(b, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+    for (int k = 0; k < 2; ++k) {
+      mask32(s[k], key0 + 64 * h + 32 * k, lim, absent >> (4 * h + 2 * k));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+        for (int c = 16 * i; c < 16 * i + 16; c += 4) {
+          a = attn::max3f(a, __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
+          b = attn::max3f(b, __uint_as_float(s[k][c + 2]), __uint_as_float(s[k][c + 3]));
+        }
+        mx = fmaxf(mx, fmaxf(a, b) * scl[4 * h + 2 * k + i]);
+      }
     }
-    mx = fmaxf(mx, fmaxf(a, b) * scl[i]);
   }
   const bool raise = mx > m_run + kTau;
   float alpha = 1.0f;
@@ -168,28 +184,29 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
     m_run = mx;
   }
   const bool rescale = o_live && __any_sync(0xffffffffu, raise);
-  const bool none = m_run == -INFINITY;
-  const float2 nm2 = make_float2(-m_run, -m_run);
-  float2 acc[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+  const float mz = m_run == -INFINITY ? 0.0f : m_run;             // a row that has seen no key: every score is -inf
+  const float2 nm2 = make_float2(-mz, -mz);
+  float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
+  for (int h = 0; h < 2; ++h) {
     uint32_t pk[32];
-    if (none) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) pk[c] = 0u;
-    } else {
+    for (int k = 0; k < 2; ++k) {
+      uint32_t s[32];
+      RL_TMEM_LD32(ta + 64 * h + 32 * k, s);
+      tmem_ld_wait_regs(s);
+      mask32(s, key0 + 64 * h + 32 * k, lim, absent >> (4 * h + 2 * k));
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const int i = 64 * hh + 2 * c;
-        const float2 sc2 = make_float2(scl[i >> 4], scl[i >> 4]);
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, nm2);
+      for (int c = 0; c < 16; ++c) {
+        const float f = scl[4 * h + 2 * k + (c >> 3)];
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), make_float2(f, f), nm2);
         const float2 e = make_float2(attn::ex2_approx(x.x), attn::ex2_approx(x.y));
-        pk[c] = kvattn::pack_h2(e.x, e.y);
-        acc[c & 3] = __fadd2_rn(acc[c & 3], e);
+        pk[16 * k + c] = kvattn::pack_h2(e.x, e.y);
+        acc[c & 1] = __fadd2_rn(acc[c & 1], e);
       }
     }
-    RL_TMEM_ST32(ta + 32 * hh, pk);
-    if (hh == 0 && rescale) {
+    RL_TMEM_ST32(ta + 32 * h, pk);
+    if (h == 0 && rescale) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -204,10 +221,9 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
     tmem_st_wait_regs(pk);
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&p_bar[hh]);
+    if (lane == 0) mbar_arrive(&p_bar[h]);
   }
-  const float2 a01 = __fadd2_rn(acc[0], acc[1]), a23 = __fadd2_rn(acc[2], acc[3]);
-  const float2 a = __fadd2_rn(a01, a23);
+  const float2 a = __fadd2_rn(acc[0], acc[1]);
   l_run += a.x + a.y;
 }
 
@@ -291,25 +307,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   const int nblk = static_cast<int>((kmax + BKV - 1) / BKV);      // >= 1
 
   if (warp < 4) {
-    attn::setmaxnreg_dec<kRegsLow>();
     if (warp != 1) {
       // ---------------- converters ----------------
       const int cw = warp == 0 ? 0 : warp - 1;
-      auto block_at = [&](int u) -> int {       // pool index of the sequence's 16-key block u; -1 beyond the keys, -2 absent
-        const int64_t pos = static_cast<int64_t>(u) * BT;
-        if (pos >= kmax) return -1;
-        const int pg = __ldg(a.batch.table + b * a.batch.ld + (pos >> a.page_sh));
-        if (static_cast<uint32_t>(pg) >= a.pool.pages) return -2;
-        return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + ((static_cast<int>(pos) & (a.pool.page - 1)) >> 4);
+      // the page of the sequence's 16-key block u (-1 beyond the keys), and the block's pool index in it
+      const int32_t* table = a.batch.table + b * a.batch.ld;
+      const int units = static_cast<int>((kmax + BT - 1) / BT);
+      auto page_of = [&](int u) -> int { return u < units ? __ldg(table + (u >> (a.page_sh - 4))) : -1; };
+      auto present = [&](int pg) -> bool { return static_cast<uint32_t>(pg) < a.pool.pages; };
+      auto block_in = [&](int pg, int u) -> int {
+        return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + (u & ((1 << (a.page_sh - 4)) - 1));
       };
       // the largest V exponent
       int e = 0;
-      const int units = static_cast<int>((kmax + BT - 1) / BT);
 #pragma unroll 4
       for (int u = cw * 32 + lane; u < units; u += kConv * 32) {
-        const int blk = block_at(u);
-        if (blk == -2) report(kErrBadArgument);
-        const int ve = blk >= 0 ? a.pool.ve[blk] : 0;
+        const int pg = page_of(u);
+        if (!present(pg)) {
+          report(kErrBadArgument);
+          continue;
+        }
+        const int ve = a.pool.ve[block_in(pg, u)];
         if (ve != 255) e = max(e, ve);
         else atomicMin(&bars->v_poison, u * BT);
       }
@@ -333,77 +351,65 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       asm volatile("bar.sync 1, 96;" ::: "memory");               // the converters' maxima are joined
       const int em = bars->e_max;
 
-      // Warp cw converts units cw, cw + 3 and cw + 6 of each block's eight. The codes of block j + 1 are copied into the
-      // raw buffer as soon as block j's have been read (each lane reads what it copied itself), so a copy has the time
-      // of a whole block; page lookups run one block further ahead.
-      uint8_t* raw = smem + kRaw + lane * 16;
-      int idx[3];
-      uint32_t ke[3], ve[3];                                      // exponents of the block in the raw buffer | 0x100 absent
+      // Warp cw converts units cw, cw + 3 and cw + 6 of each block's eight. The codes of block j + 1 are loaded into
+      // registers as soon as block j's have been converted, so a load has the time of a whole block; page lookups run
+      // one block further ahead.
+      Unit ku[3], vu[3];
+      int pg[3];                                                  // pages of the next block's units
       auto lookup = [&](int j) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) idx[i] = j < nblk && cw + 3 * i < 8 ? block_at(j * 8 + cw + 3 * i) : -1;
+        for (int i = 0; i < 3; ++i) pg[i] = page_of(j < nblk ? j * 8 + cw + 3 * i : units);
       };
-      auto copy = [&](int v, uint32_t (&e)[3]) {
-        const uint8_t* codes = v ? a.pool.v : a.pool.k;
-        const uint8_t* exps = v ? a.pool.ve : a.pool.ke;
+      auto load = [&](const uint8_t* codes, const uint8_t* exps, int j, Unit (&u)[3]) {
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          const int64_t blk = max(idx[i], 0);                     // beyond the keys, or absent: any block, with weight zero
-          e[i] = (idx[i] < 0 ? 0u : exps[blk]) | (idx[i] == -2 ? 0x100u : 0u);
-          if (cw + 3 * i < 8) {
-            const uint8_t* p = codes + blk * (BT * HD);
-            const uint32_t d = smem_u32(raw) + v * RAW + (cw + 3 * i) * (BT * HD);
+          const int k = cw + 3 * i;
+          const bool in = present(pg[i]);
+          const int64_t blk = in ? block_in(pg[i], j * 8 + k) : 0;   // beyond the keys, or absent: any block, of weight zero
+          u[i].e = in ? exps[blk] : 0x100u;
+          const uint8_t* p = codes + blk * (BT * HD) + unit_row(0, lane) * HD + unit_code(0, lane);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) kvattn::cp_async16(d + 512 * k, p + unit_row(k, lane) * HD + unit_code(k, lane));
-          }
+          for (int y = 0; y < 4; ++y) u[i].c[y] = *reinterpret_cast<const uint4*>(p + 8 * (y >> 1) * HD + 64 * (y & 1));
         }
-        kvattn::cp_commit();
       };
       lookup(0);
-      copy(0, ke);
-      copy(1, ve);
+      load(a.pool.k, a.pool.ke, 0, ku);
+      load(a.pool.v, a.pool.ve, 0, vu);
       lookup(1);
       for (int j = 0; j < nblk; ++j) {
         const int ks = j % KS, vs = j % VS;
         if (!mbar_wait_warp(&bars->k_empty[ks], ((j / KS) & 1) ^ 1, abort)) break;
-        kvattn::cp_wait<1>();
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const int k = cw + 3 * i;
-          if (k < 8) {
-            write_unit<false>(smem + kK + ks * TILE, 16 * k, raw + k * (BT * HD), 0x7F007F00u, 0xC000C000u, lane);
-            if (lane == 0) {                                      // (the last use of this slot was eight blocks ago)
-              const bool poisoned = ke[i] == 255u;
-              bars->scale[j % RING][k] = poisoned ? 1.0f : bfp16_scale(ke[i] & 255u) * 64.0f * a.scale_log2;
-              bars->flag[j % RING][k] = static_cast<uint8_t>((poisoned ? 1 : 0) | (ke[i] & 0x100u ? 2 : 0));
-            }
-          }
+        for (int i = 0; i < 3; ++i)
+          if (cw + 3 * i < 8) write_unit<false>(smem + kK + ks * TILE, 16 * (cw + 3 * i), ku[i], 0x7F007F00u, 0xC000C000u, lane);
+        if (lane < 3 && cw + 3 * lane < 8) {                      // (the last use of this slot was eight blocks ago)
+          const uint32_t e = lane == 0 ? ku[0].e : lane == 1 ? ku[1].e : ku[2].e;
+          // (never zero: a masked score is -inf times this)
+          bars->scale[j % RING][cw + 3 * lane] =
+              e == 255u ? 1.0f : fmaxf(bfp16_scale(e & 255u) * 64.0f * a.scale_log2, 1.17549435e-38f);
+          bars->flag[j % RING][cw + 3 * lane] = static_cast<uint8_t>((e == 255u ? 1 : 0) | (e & 0x100u ? 2 : 0));
         }
+        load(a.pool.k, a.pool.ke, j + 1, ku);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->k_full[ks]);
-        copy(0, ke);
         if (!mbar_wait_warp(&bars->v_empty[vs], ((j / VS) & 1) ^ 1, abort)) break;
-        kvattn::cp_wait<1>();
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          const int k = cw + 3 * i;
-          if (k < 8) {
-            // 2^-d and -1152 2^-d in fp16. Keys beyond the end or absent have exponent 0: d > 24 unless all are near 0,
-            // and P = 0 in any case; a poisoned block's codes count as they are (the rows that see it become NaN).
-            const int d = em - static_cast<int>(ve[i] & 255u);
-            const float f = d < 0 ? 1.0f : d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
-            write_unit<true>(smem + kV + vs * TILE, 16 * k, raw + RAW + k * (BT * HD), kvattn::pack_h2(f, f),
+          // 2^-d and -1152 2^-d in fp16. P = 0 for keys beyond the end or absent; a poisoned block's codes count as
+          // they are (the rows that see it become NaN).
+          const int d = vu[i].e == 255u ? 0 : em - static_cast<int>(vu[i].e & 255u);
+          const float f = d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
+          if (cw + 3 * i < 8)
+            write_unit<true>(smem + kV + vs * TILE, 16 * (cw + 3 * i), vu[i], kvattn::pack_h2(f, f),
                              kvattn::pack_h2(-1152.0f * f, -1152.0f * f), lane);
-          }
         }
+        load(a.pool.v, a.pool.ve, j + 1, vu);
+        lookup(j + 2);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->v_full[vs]);
-        copy(1, ve);
-        lookup(j + 2);
       }
-      kvattn::cp_wait<0>();
     } else {
       // ---------------- MMA issuer (warp-wide, elected lane issues) ----------------
       constexpr uint32_t idesc_s = idesc_bf16(BQ, BKV);
@@ -461,7 +467,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       __syncwarp();
     }
   } else {
-    attn::setmaxnreg_inc<kRegsHigh>();
     // ---------------- softmax of tile t (thread = row = TMEM lane) ----------------
     const int t = (warp - 4) >> 2, q = warp & 3;
     const uint32_t row = row0 + t * BQ + 32 * q + lane;
@@ -519,16 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   }
 }
 
-// The register split waits for registers that the launch must have brought (see rl_attn.cu): checked once per device.
 inline int launch(int64_t tasks, const Args& a, cudaStream_t stream) {
-  static int regs = 0;
-  if (regs == 0) {
-    cudaFuncAttributes fa;
-    RL_TRY_CUDA(cudaFuncGetAttributes(&fa, prompt_kernel));
-    regs = fa.numRegs;
-  }
-  RL_REQUIRE(regs == kRegsLaunch, RL_ERR_UNSUPPORTED, "rl_kv_attention: compiled with %d registers a thread, its register "
-             "split needs %d", regs, kRegsLaunch);
   RL_TRY_CUDA(cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
   prompt_kernel<<<static_cast<unsigned>(tasks), kThreads, kBytes, stream>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
