@@ -122,59 +122,43 @@ __device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u,
   }
 }
 
-// What hides a score of the 32 columns from `c0`: keys beyond the row's limit, and blocks of absent pages.
-__device__ __forceinline__ void mask32(uint32_t (&s)[32], int key, int lim, uint32_t absent) {
-  if (key + 31 > lim) {
-#pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (key + c > lim) s[c] = 0xFF800000u;  // -inf
-  }
-  if (absent) {
-#pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (absent >> (c >> 4) & 1) s[c] = 0xFF800000u;
-  }
-}
-
-// One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys. S
-// is read from TMEM twice, 32 columns at a time, for the maximum and for the exponentials: holding the row would take 128
-// registers of every softmax thread. P of columns c .. is written to the first half of columns that were read before.
+// One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys.
 __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0, int lim, const float* scale,
                                               uint2 flags, bool o_live, float& m_run, float& l_run, uint64_t* p_bar,
                                               int lane) {
-  uint32_t absent = 0;   // bit i: 16-key block i
+  uint32_t s[BKV];
+#pragma unroll
+  for (int c = 0; c < BKV / 32; ++c) {
+    uint32_t (&sc)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]);
+    RL_TMEM_LD32(ta + 32 * c, sc);
+  }
+  tmem_ld_wait_regs(s);
+  if (key0 + BKV - 1 > lim) {
+#pragma unroll
+    for (int c = 0; c < BKV; ++c)
+      if (key0 + c > lim) s[c] = 0xFF800000u;  // -inf
+  }
   if (flags.x | flags.y) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t f = (i < 4 ? flags.x : flags.y) >> (8 * (i & 3));
-      absent |= (f >> 1 & 1) << i;
+      if (f & 2) {
+#pragma unroll
+        for (int c = 16 * i; c < 16 * i + 16; ++c) s[c] = 0xFF800000u;
+      }
       if ((f & 1) && key0 + 16 * i <= lim) l_run = __uint_as_float(0x7FC00000u);
     }
   }
-  const float4 sa = *reinterpret_cast<const float4*>(scale), sb = *reinterpret_cast<const float4*>(scale + 4);
-  const float scl[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
   float mx = -INFINITY;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t s[2][32];
-    RL_TMEM_LD32(ta + 64 * h, s[0]);
-    RL_TMEM_LD32(ta + 64 * h + 32, s[1]);
-    tmem_ld_wait_regs(s[0]);
-    tmem_ld_wait_regs(s[1]);
+  for (int i = 0; i < 8; ++i) {
+    float a = -INFINITY, b = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      mask32(s[k], key0 + 64 * h + 32 * k, lim, absent >> (4 * h + 2 * k));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-        for (int c = 16 * i; c < 16 * i + 16; c += 4) {
-          a = attn::max3f(a, __uint_as_float(s[k][c]), __uint_as_float(s[k][c + 1]));
-          b = attn::max3f(b, __uint_as_float(s[k][c + 2]), __uint_as_float(s[k][c + 3]));
-        }
-        mx = fmaxf(mx, fmaxf(a, b) * scl[4 * h + 2 * k + i]);
-      }
+    for (int c = 16 * i; c < 16 * i + 16; c += 4) {
+      a = attn::max3f(a, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+      b = attn::max3f(b, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
     }
+    mx = fmaxf(mx, fmaxf(a, b) * scale[i]);
   }
   const bool raise = mx > m_run + kTau;
   float alpha = 1.0f;
@@ -191,30 +175,27 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
   for (int h = 0; h < 2; ++h) {
     uint32_t pk[32];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t s[32];
-      RL_TMEM_LD32(ta + 64 * h + 32 * k, s);
-      tmem_ld_wait_regs(s);
-      mask32(s, key0 + 64 * h + 32 * k, lim, absent >> (4 * h + 2 * k));
+    for (int g = 0; g < 4; ++g) {
+      const float f = scale[4 * h + g];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float f = scl[4 * h + 2 * k + (c >> 3)];
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), make_float2(f, f), nm2);
+      for (int c = 0; c < 8; ++c) {
+        const int i = 64 * h + 16 * g + 2 * c;
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(f, f), nm2);
         const float2 e = make_float2(attn::ex2_approx(x.x), attn::ex2_approx(x.y));
-        pk[16 * k + c] = kvattn::pack_h2(e.x, e.y);
+        pk[8 * g + c] = kvattn::pack_h2(e.x, e.y);
         acc[c & 1] = __fadd2_rn(acc[c & 1], e);
       }
     }
     RL_TMEM_ST32(ta + 32 * h, pk);
     if (h == 0 && rescale) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        RL_TMEM_LD32(to + 32 * c, o);
+      for (int c = 0; c < 8; ++c) {
+        uint32_t o[16];
+        RL_TMEM_LD16(to + 16 * c, o);
         tmem_ld_wait_regs(o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-        RL_TMEM_ST32(to + 32 * c, o);
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        RL_TMEM_ST16(to + 16 * c, o);
         tmem_st_wait_regs(o);
       }
     }
