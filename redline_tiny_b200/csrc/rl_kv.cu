@@ -51,9 +51,10 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b, int page) {
 
 // Index of the block (layer-wide) that holds token position `pos` of sequence b for head h, or -1 for a bad page.
 __device__ __forceinline__ int64_t block_index(const Pool& p, const Batch& bt, int b, int64_t pos, int h) {
-  const int64_t pg = __ldg(bt.table + b * bt.ld + pos / p.page);
+  const int sh = 31 - __clz(p.page);                                 // the page size is a power of two
+  const int64_t pg = __ldg(bt.table + b * bt.ld + (pos >> sh));
   if (pg < 0 || pg >= p.pages) return -1;
-  return (pg * p.hkv + h) * (p.page / BT) + (pos % p.page) / BT;
+  return ((pg * p.hkv + h) << (sh - 4)) + ((pos & (p.page - 1)) >> 4);
 }
 
 // m / 2^d for a code of an older token, rounded half to even (d >= 1), as an offset-binary byte.
@@ -63,38 +64,111 @@ __device__ __forceinline__ uint32_t shift_code(uint32_t u, int d) {
   return static_cast<uint32_t>(((m + (1 << (d - 1)) - 1 + ((m >> d) & 1)) >> d) + 128);
 }
 
+// Codes of four new values (float32 bits) under exponent E: min(rint_half_even(x 2^(133 - E)), 127) + 128 as bytes. E is
+// no smaller than the values' own exponent fields, so |x 2^(133 - E)| < 128 and only + 128 has to be clipped. The rounding is
+// one FMA against 1.5 * 2^23, whose low byte is then the code but for its top bit; exponents near the ends of the range
+// take the integer form.
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t E) {
+  if (E >= 7u && E < 255u) {
+    constexpr float kMagic = 12582912.0f;
+    const float s = __uint_as_float((260u - E) << 23);
+    auto q = [&](uint32_t x) { return __float_as_uint(fminf(fmaf(__uint_as_float(x), s, kMagic), kMagic + 127.0f)); };
+    return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410) ^ 0x80808080u;
+  }
+  auto q = [&](uint32_t x) { return static_cast<uint32_t>(bfp16_quant_one(x, E) + 128); };
+  return q(a) | q(b) << 8 | q(c) << 16 | q(d) << 24;
+}
+
 struct Source {             // rows of new keys or values: element (t, h, d) at t * st + h * sh + d * sd
   const void* x;
   int64_t st, sh, sd;
 };
 
-// The 4 values of one token that a lane owns (dims 4 * lane ..), as float32 bits.
+// The new values of a block in a warp's registers: up to 16 tokens x 128 dims.
+//
+// Any type and strides: lane l holds dims 4 l .. + 3 of every token, as float32 bits.
 template <typename X>
-__device__ __forceinline__ void load4(const Source& s, int64_t t, int h, int lane, bool vec, uint32_t (&b)[4]) {
-  const X* p = static_cast<const X*>(s.x) + t * s.st + h * s.sh + 4 * lane * s.sd;
-  if (sizeof(X) == 2) {
-    if (vec) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      b[0] = w.x << 16, b[1] = w.x & 0xFFFF0000u, b[2] = w.y << 16, b[3] = w.y & 0xFFFF0000u;
-    } else {
+struct AnyBlock {
+  uint32_t x[BT][4];
+  __device__ __forceinline__ void load(const Source& s, int64_t t0, int cnt, int h, int lane) {
+    const bool vec = s.sd == 1 && ((reinterpret_cast<uintptr_t>(s.x) | (s.st * sizeof(X)) | (s.sh * sizeof(X))) &
+                                   (4 * sizeof(X) - 1)) == 0;
+    const X* p0 = static_cast<const X*>(s.x) + t0 * s.st + h * s.sh + 4 * lane * s.sd;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + i * s.sd)) << 16;
-    }
-  } else {
-    if (vec) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
-    } else {
+    for (int t = 0; t < BT; ++t) {
+      x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0u;
+      if (t >= cnt) continue;
+      const X* p = p0 + t * s.st;
+      if (sizeof(X) == 2) {
+        if (vec) {
+          const uint2 w = *reinterpret_cast<const uint2*>(p);
+          x[t][0] = w.x << 16, x[t][1] = w.x & 0xFFFF0000u, x[t][2] = w.y << 16, x[t][3] = w.y & 0xFFFF0000u;
+        } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint32_t*>(p + i * s.sd);
+          for (int i = 0; i < 4; ++i) x[t][i] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + i * s.sd)) << 16;
+        }
+      } else {
+        if (vec) {
+          const uint4 w = *reinterpret_cast<const uint4*>(p);
+          x[t][0] = w.x, x[t][1] = w.y, x[t][2] = w.z, x[t][3] = w.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[t][i] = *reinterpret_cast<const uint32_t*>(p + i * s.sd);
+        }
+      }
     }
   }
-}
+  __device__ __forceinline__ uint32_t exponent() const {
+    uint32_t mx = 0;
+#pragma unroll
+    for (int t = 0; t < BT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = max(mx, x[t][i] & 0x7FFFFFFFu);
+    return __reduce_max_sync(0xffffffffu, mx) >> 23;
+  }
+  __device__ __forceinline__ void store(uint8_t* row, int cnt, uint32_t E, int lane) const {
+    uint32_t* p = reinterpret_cast<uint32_t*>(row) + lane;
+#pragma unroll
+    for (int t = 0; t < BT; ++t)
+      if (t < cnt) p[t * (HD / 4)] = codes4(x[t][0], x[t][1], x[t][2], x[t][3], E);
+  }
+};
+
+// bf16 rows at 16-byte boundaries: lanes 0 - 15 hold the even tokens and 16 - 31 the odd ones, 8 dims each. Half the
+// registers of the form above and loads of 16 bytes: 26.4 -> 12.6 us for 8321 tokens of 8 heads.
+struct WideBlock {
+  uint4 x[BT / 2];
+  __device__ __forceinline__ void load(const Source& s, int64_t t0, int cnt, int h, int lane) {
+    const uint16_t* p = static_cast<const uint16_t*>(s.x) + (t0 + (lane >> 4)) * s.st + h * s.sh + 8 * (lane & 15);
+#pragma unroll
+    for (int t = 0; t < BT / 2; ++t) {
+      x[t] = make_uint4(0, 0, 0, 0);
+      if (2 * t + (lane >> 4) < cnt) x[t] = __ldcs(reinterpret_cast<const uint4*>(p + 2 * t * s.st));
+    }
+  }
+  __device__ __forceinline__ uint32_t exponent() const {
+    uint32_t m = 0;                                         // two 16-bit maxima
+#pragma unroll
+    for (int t = 0; t < BT / 2; ++t) {
+      m = __vmaxu2(m, x[t].x & 0x7FFF7FFFu), m = __vmaxu2(m, x[t].y & 0x7FFF7FFFu);
+      m = __vmaxu2(m, x[t].z & 0x7FFF7FFFu), m = __vmaxu2(m, x[t].w & 0x7FFF7FFFu);
+    }
+    return __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16)) >> 7;
+  }
+  __device__ __forceinline__ void store(uint8_t* row, int cnt, uint32_t E, int lane) const {
+    uint2* p = reinterpret_cast<uint2*>(row + (lane >> 4) * HD) + (lane & 15);
+#pragma unroll
+    for (int t = 0; t < BT / 2; ++t)
+      if (2 * t + (lane >> 4) < cnt)
+        p[t * (2 * HD / 8)] = make_uint2(codes4(x[t].x << 16, x[t].x & 0xFFFF0000u, x[t].y << 16, x[t].y & 0xFFFF0000u, E),
+                                         codes4(x[t].z << 16, x[t].z & 0xFFFF0000u, x[t].w << 16, x[t].w & 0xFFFF0000u, E));
+  }
+};
 
 // One warp per (group of `rows` rows, head, K or V). A row leads when it is the first of its block among the new
 // tokens; the warp writes the blocks of its leading rows: the block's new values are read once into registers, their
 // largest exponent field is joined with the exponent of the older tokens of the block, and the codes are stored.
-template <typename X>
+template <typename Block>
 __global__ void __launch_bounds__(128) append_kernel(const Source sk, const Source sv, const Pool p, const Batch bt,
                                                      int rows, int64_t groups) {
   const int lane = threadIdx.x & 31;
@@ -106,8 +180,6 @@ __global__ void __launch_bounds__(128) append_kernel(const Source sk, const Sour
   const Source src = is_v ? sv : sk;
   uint8_t* codes = is_v ? p.v : p.k;
   uint8_t* exps = is_v ? p.ve : p.ke;
-  const bool vec = src.sd == 1 && ((reinterpret_cast<uintptr_t>(src.x) | (src.st * sizeof(X)) | (src.sh * sizeof(X))) &
-                                   (4 * sizeof(X) - 1)) == 0;
   // the sequence of row r0: the last b with q_start[b] <= r0
   int lo = 0, hi = bt.B;
   while (hi - lo > 1) {
@@ -131,109 +203,78 @@ __global__ void __launch_bounds__(128) append_kernel(const Source sk, const Sour
       continue;
     }
     const int cnt = static_cast<int>(min(static_cast<int64_t>(BT - a), s.s0 + s.n - r));
+    Block x;
+    x.load(src, r, cnt, h, lane);
     const int64_t blk = block_index(p, bt, b, pos, h);
     if (blk < 0) {
       if (lane == 0) report(kErrBadArgument);
       r += cnt;
       continue;
     }
-    uint32_t x[BT][4];
-    uint32_t mx = 0;
-#pragma unroll
-    for (int t = 0; t < BT; ++t) {
-      if (t < cnt) {
-        load4<X>(src, r + t, h, lane, vec, x[t]);
-      } else {
-        x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0u;
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < BT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx = max(mx, x[t][i] & 0x7FFFFFFFu);
-    uint32_t E = __reduce_max_sync(0xffffffffu, mx) >> 23;
-    uint32_t* row = reinterpret_cast<uint32_t*>(codes + blk * (BT * HD)) + lane;
+    uint32_t E = x.exponent();
+    uint8_t* row = codes + blk * (BT * HD);
     if (a > 0) {
       const uint32_t Eo = exps[blk];
       if (Eo >= E) {
         E = Eo;
       } else {
         const int d = static_cast<int>(E - Eo);
+        uint32_t* old = reinterpret_cast<uint32_t*>(row) + lane;
         for (int t = 0; t < a; ++t) {
-          const uint32_t u = row[t * (HD / 4)];
-          row[t * (HD / 4)] = shift_code(u & 255u, d) | (shift_code(u >> 8 & 255u, d) << 8) |
+          const uint32_t u = old[t * (HD / 4)];
+          old[t * (HD / 4)] = shift_code(u & 255u, d) | (shift_code(u >> 8 & 255u, d) << 8) |
                               (shift_code(u >> 16 & 255u, d) << 16) | (shift_code(u >> 24, d) << 24);
         }
       }
       __syncwarp();   // every lane has read the exponent before lane 0 replaces it
     }
-    if (E >= 7u && E < 255u) {
-      // rint_half_even(x * 2^(133 - E)) by one FMA against 1.5 * 2^23, clamped to the code range
-      constexpr float kMagic = 12582912.0f;
-      const float sc = __uint_as_float((260u - E) << 23);
-#pragma unroll
-      for (int t = 0; t < BT; ++t) {
-        if (t < cnt) {
-          uint32_t u = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float m = fminf(fmaxf(__fsub_rn(fmaf(__uint_as_float(x[t][i]), sc, kMagic), kMagic), -128.0f), 127.0f);
-            u |= (__float_as_uint(__fadd_rn(m, kMagic + 128.0f)) & 0xFFu) << (8 * i);
-          }
-          row[(a + t) * (HD / 4)] = u;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BT; ++t) {
-        if (t < cnt) {
-          uint32_t u = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) u |= static_cast<uint32_t>(bfp16_quant_one(x[t][i], E) + 128) << (8 * i);
-          row[(a + t) * (HD / 4)] = u;
-        }
-      }
-    }
+    x.store(row + a * HD, cnt, E, lane);
     if (lane == 0) exps[blk] = static_cast<uint8_t>(E);
     r += cnt;
   }
 }
 
-// One thread per 8 values of the output (B, count, Hkv, 128): token start[b] + i of sequence b, zero at and after its
-// length (and on a bad page, which is reported).
-__global__ void __launch_bounds__(256) read_kernel(const Pool p, const int32_t* table, int64_t ld, const int32_t* kv_len,
-                                                   const int32_t* start, int B, int64_t count, uint16_t* ko, uint16_t* vo) {
-  const int64_t per = count * p.hkv * (HD / 8);
-  const int64_t total = per * B;
-  Batch bt{table, ld, kv_len, nullptr, B, 0};
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int b = static_cast<int>(i / per);
-    const int64_t rem = i - b * per;
-    const int64_t tok = rem / (p.hkv * (HD / 8));
-    const int h = static_cast<int>(rem / (HD / 8) % p.hkv), c = static_cast<int>(rem % (HD / 8));
-    const int64_t pos = __ldg(start + b) + tok;
-    const int64_t len = __ldg(kv_len + b);
-    uint32_t wk[4] = {0, 0, 0, 0}, wv[4] = {0, 0, 0, 0};
-    if (pos >= 0 && pos < len) {
-      const int64_t blk = pos < ld * p.page ? block_index(p, bt, b, pos, h) : -1;
-      if (blk < 0) {
-        report(kErrBadArgument);
-      } else {
-        const int64_t off = blk * (BT * HD) + (pos % BT) * HD + c * 8;
-        const uint2 uk = *reinterpret_cast<const uint2*>(p.k + off), uv = *reinterpret_cast<const uint2*>(p.v + off);
-        const uint32_t ek = p.ke[blk], ev = p.ve[blk];
-        bfp16_decode_block_ob(ek, uk.x, uk.y, wk);
-        bfp16_decode_block_ob(ev, uv.x, uv.y, wv);
+// Two 16-byte stores of decoded values per 16 codes.
+__device__ __forceinline__ void decode16(const uint4& u, uint32_t e, uint16_t* out) {
+  uint32_t w[2][4];
+  bfp16_decode_block_ob(e, u.x, u.y, w[0]);
+  bfp16_decode_block_ob(e, u.z, u.w, w[1]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (ek == 255u) wk[q] = 0x7FC07FC0u;
-          if (ev == 255u) wv[q] = 0x7FC07FC0u;
-        }
-      }
+  for (int i = 0; i < 2; ++i) {
+    const bool nan = e == 255u;
+    __stcs(reinterpret_cast<uint4*>(out) + i, nan ? make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u)
+                                                  : make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+  }
+}
+
+// One thread per 16 values of the output (B, count, Hkv, 128), blockIdx.y = the sequence: token start[b] + i of sequence
+// b, zero at and after its length (and on a bad page, which is reported).
+__global__ void __launch_bounds__(256) read_kernel(const Pool p, const int32_t* table, int64_t ld, const int32_t* kv_len,
+                                                   const int32_t* start, uint32_t count, uint16_t* ko, uint16_t* vo) {
+  const int b = blockIdx.y;
+  const uint32_t per = count * p.hkv * (HD / 16);
+  const int64_t base = static_cast<int64_t>(b) * per;
+  const int64_t first = __ldg(start + b), len = __ldg(kv_len + b);
+  const Batch bt{table, ld, kv_len, nullptr, 0, 0};
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < per; i += gridDim.x * blockDim.x) {
+    const uint32_t c = i % (HD / 16), th = i / (HD / 16), tok = th / p.hkv;
+    const int h = static_cast<int>(th - tok * p.hkv);
+    const int64_t pos = first + tok;
+    uint16_t* k = ko + (base + i) * 16;
+    uint16_t* v = vo + (base + i) * 16;
+    const bool in = pos >= 0 && pos < len;
+    const int64_t blk = in && pos < ld * p.page ? block_index(p, bt, b, pos, h) : -1;
+    if (in && blk < 0) report(kErrBadArgument);
+    if (blk < 0) {
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      __stcs(reinterpret_cast<uint4*>(k), z), __stcs(reinterpret_cast<uint4*>(k) + 1, z);
+      __stcs(reinterpret_cast<uint4*>(v), z), __stcs(reinterpret_cast<uint4*>(v) + 1, z);
+    } else {
+      const int64_t off = blk * (BT * HD) + (pos % BT) * HD + c * 16;
+      const uint4 uk = *reinterpret_cast<const uint4*>(p.k + off), uv = *reinterpret_cast<const uint4*>(p.v + off);
+      decode16(uk, p.ke[blk], k);
+      decode16(uv, p.ve[blk], v);
     }
-    *reinterpret_cast<uint4*>(ko + i * 8) = make_uint4(wk[0], wk[1], wk[2], wk[3]);
-    *reinterpret_cast<uint4*>(vo + i * 8) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
   }
 }
 
@@ -341,10 +382,14 @@ int rl_kv_append(const void* k, int64_t k_st, int64_t k_sh, int64_t k_sd, const 
   const int64_t groups = (T + rows - 1) / rows;
   const int64_t ctas = (groups * kv_heads * 2 + 3) / 4;
   const kv::Source sk{k, k_st, k_sh, k_sd}, sv{v, v_st, v_sh, v_sd};
-  if (dtype == RL_BF16)
-    kv::append_kernel<uint16_t><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
+  auto wide = [](const kv::Source& s) { return s.sd == 1 && aligned(s.x, 16) && s.st % 8 == 0 && s.sh % 8 == 0; };
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (dtype == RL_BF16 && wide(sk) && wide(sv))
+    kv::append_kernel<kv::WideBlock><<<grid, 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
+  else if (dtype == RL_BF16)
+    kv::append_kernel<kv::AnyBlock<uint16_t>><<<grid, 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
   else
-    kv::append_kernel<float><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
+    kv::append_kernel<kv::AnyBlock<float>><<<grid, 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
   RL_TRY_CUDA(cudaGetLastError());
   return RL_OK;
 }
@@ -358,16 +403,16 @@ int rl_kv_read(const uint8_t* pool_k, const uint8_t* pool_v, const uint8_t* pool
   const kv::Batch bt{table, table_ld, kv_len, nullptr, B, 0};
   int st;
   if ((st = kv::check_pool("rl_kv_read", p)) != RL_OK || (st = kv::check_batch("rl_kv_read", bt)) != RL_OK) return st;
-  RL_REQUIRE(count >= 0 && count <= (1 << 28), RL_ERR_ARGUMENT, "rl_kv_read: count %lld", (long long)count);
+  RL_REQUIRE(count >= 0 && count * kv_heads <= (1 << 27), RL_ERR_ARGUMENT, "rl_kv_read: count %lld of %d heads",
+             (long long)count, kv_heads);
   if (count == 0 || B == 0) return RL_OK;
   RL_REQUIRE(start && k_out && v_out, RL_ERR_ARGUMENT, "rl_kv_read: NULL pointer");
   RL_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(start, 4), RL_ERR_ALIGNMENT,
              "rl_kv_read: outputs must be 16-byte aligned");
   RL_REQUIRE(device_is_sm100(), RL_ERR_UNSUPPORTED, "rl_kv_read: needs an sm_100 device");
-  const int64_t work = static_cast<int64_t>(B) * count * kv_heads * (kv::HD / 8);
-  const int64_t ctas = (work + 255) / 256, most = static_cast<int64_t>(sm_count()) * 64;
-  kv::read_kernel<<<static_cast<unsigned>(ctas < most ? ctas : most), 256, 0, stream>>>(p, table, table_ld, kv_len,
-                                                                                         start, B, count, k_out, v_out);
+  const int64_t ctas = (count * kv_heads * (kv::HD / 16) + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(ctas), static_cast<unsigned>(B));
+  kv::read_kernel<<<grid, 256, 0, stream>>>(p, table, table_ld, kv_len, start, static_cast<uint32_t>(count), k_out, v_out);
   RL_TRY_CUDA(cudaGetLastError());
   return RL_OK;
 }
