@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/redline_b200.h"
 
 namespace rl {
@@ -22,6 +24,23 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_tiled();
+
+// Work to be done once per device (a function's attributes); a failed attempt is repeated by the next call. The worst that
+// two threads at once can do is to do it twice.
+struct PerDevice {
+  std::atomic<bool> done[64] = {};
+  template <typename F>
+  cudaError_t once(F f) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return f();
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = f();
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+    return e;
+  }
+};
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

@@ -647,8 +647,11 @@ template <int NT>
 inline int launch(const Args& a, cudaStream_t st) {
   const size_t smem = Cfg<NT>::smem(a.batch.B);
   const int ctas = ctas_of(NT);
-  RL_TRY_CUDA(cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch))));
+  static PerDevice ready;
+  RL_TRY_CUDA(ready.once([] {
+    return cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch)));
+  }));
   attend_kernel<NT><<<ctas, Cfg<NT>::kThreads, smem, st>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};

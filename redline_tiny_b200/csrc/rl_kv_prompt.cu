@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
 }
 
 inline int launch(int64_t tasks, const Args& a, cudaStream_t stream) {
-  RL_TRY_CUDA(cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  static PerDevice ready;
+  RL_TRY_CUDA(ready.once([] { return cudaFuncSetAttribute(prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes); }));
   prompt_kernel<<<static_cast<unsigned>(tasks), kThreads, kBytes, stream>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
   return RL_OK;

@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(Many<NT>::kThreads, Many<NT>::kCtas) many_kern
 template <int NT, int G, bool kSwiglu>
 inline int launch_many(const Args& a, cudaStream_t s) {
   auto kern = many_kernel<NT, G, kSwiglu>;
-  RL_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<NT>::kSmem));
+  static PerDevice ready;
+  RL_TRY_CUDA(ready.once([=] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<NT>::kSmem); }));
   // shares of K: as many as keep the grid within the GPU's resident CTAs and leave each at least two k tiles
   const int64_t groups = (a.N + Many<NT>::kCols - 1) / Many<NT>::kCols, kt = tiles_k(a.K);
   const int64_t slots = static_cast<int64_t>(sm_count()) * Many<NT>::kCtas;

@@ -310,12 +310,17 @@ def conv2d(x_dq, w, bias, taps, out=None):
 
 def _here(*ts):
     """The current device's index, after checking that the tensors (None allowed) lie on it."""
-    dev = torch.cuda.current_device()
+    dev = None
     for t in ts:
-        if t is not None and t.get_device() != dev:
-            if not t.is_cuda:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
                 raise ValueError("redline_tiny_b200 ops take CUDA tensors (no CPU path)")
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+            dev = torch._C._cuda_getDevice()
+            if d != dev:
+                raise ValueError(f"tensor on cuda:{d}, but the current device is cuda:{dev}")
     return dev
 
 
@@ -367,9 +372,13 @@ def _batch(table, kv_len, starts, extra):
     if table.dim() != 2 or table.shape[1] == 0:
         raise ValueError("table must be int32 (sequences, pages)")
     B, width = table.shape
-    _check_int32("table", table, B, width)
-    _check_int32("kv_len", kv_len, B)
-    _check_int32("q_start" if extra else "start", starts, B + extra)
+    i32 = torch.int32
+    if not (table.dtype is i32 and kv_len.dtype is i32 and starts.dtype is i32 and table.is_contiguous()
+            and kv_len.is_contiguous() and starts.is_contiguous() and kv_len.shape == (B,)
+            and starts.shape == (B + extra,)):
+        _check_int32("table", table, B, width)
+        _check_int32("kv_len", kv_len, B)
+        _check_int32("q_start" if extra else "start", starts, B + extra)
     return B, width
 
 
@@ -442,10 +451,10 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     if row_limit is not None:
         _check_int32("row_limit", row_limit, T)
     if out is None:
-        out = torch.empty((T, H * 128), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((T, H * 128))
     elif out.dtype is not torch.bfloat16 or out.shape != (T, H * 128) or out.stride(1) != 1:
         raise ValueError(f"out must be bf16 ({T}, {H * 128}) with contiguous rows")
-    ws = torch.empty(_kv_attention_workspace(dev, T, B, H, pool.kv_heads), dtype=torch.uint8, device=q.device)
+    ws = pool.k.new_empty(_kv_attention_workspace(dev, T, B, H, pool.kv_heads))
     L.call("rl_kv_attention", q.data_ptr(), st, sh, T, H, *pool._args(layer), table.data_ptr(), width,
            kv_len.data_ptr(), q_start.data_ptr(), B, None if row_limit is None else row_limit.data_ptr(),
            _SCALE_LOG2 if scale_log2 is None else scale_log2, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
@@ -501,14 +510,15 @@ def quantize_w4(B, group=64):
 
 def _w4(x, w, bias, epi, out, cols, out_dtype):
     dev = _here(x, w.codes, bias, out)
-    _check_cuda(x, bias, out)
     M = x.shape[0]
     if x.shape != (M, w.K) or x.dtype is not torch.bfloat16:
         raise ValueError(f"x must be bf16 (rows, {w.K}), not {x.dtype} {tuple(x.shape)}")
+    if not x.is_contiguous() or (bias is not None and not bias.is_contiguous()) or (out is not None and not out.is_contiguous()):
+        raise ValueError("tensor must be contiguous")
     if bias is not None and (bias.dtype is not torch.bfloat16 or bias.shape != (w.N,)):
         raise ValueError(f"bias must be bf16 ({w.N},)")
     if out is None:
-        out = torch.empty((M, cols), dtype=out_dtype, device=x.device)
+        out = x.new_empty((M, cols), dtype=out_dtype)
     elif out.shape != (M, cols):
         raise ValueError(f"out must be {(M, cols)}")
     L.call("rl_linear_w4", x.data_ptr(), M, w.K, *w._ptrs, w.N, w.group, None if bias is None else bias.data_ptr(), epi,

@@ -97,3 +97,63 @@ def test_w4_sizes(lib):
     assert (cb.value, sb.value) == (3 * 2 * 1024, 3 * 8 * 16 * 2)     # N padded to 48, K to 256
     refused(lib, "rl_w4_bytes", (160, 33, 64, 0, ctypes.byref(cb), ctypes.byref(sb)), -1, b"multiple")
     refused(lib, "rl_linear_w4", (P + 2, 1, 64, P, P, 16, 32, None, 0, P, 1, None), -2, b"aligned")
+
+
+def test_host_tensors_are_refused():
+    """The Python layer turns down tensors in host memory before their addresses reach a kernel, whichever argument they
+    are, and tells a wrong type or shape from them."""
+    torch = pytest.importorskip("torch")
+    from redline_tiny_b200 import ops
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+
+    class OnDevice:   # a tensor that claims to lie on a device
+        def __init__(self, *shape, dtype=bf):
+            self.t = torch.zeros(shape, dtype=dtype)
+
+        def get_device(self):
+            return 0
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    codes, exps = torch.full((1, 4, 2, 16, 128), 128, dtype=u8), torch.zeros((1, 4, 2, 1), dtype=u8)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.KVPool(codes, codes, exps, exps)
+    pool = ops.KVPool.__new__(ops.KVPool)
+    pool.k, pool.layers, pool.pages, pool.kv_heads, pool.page, pool._ptrs = codes, 1, 4, 2, 16, [(0, 0, 0, 0)]
+    table, lens, start = torch.zeros((1, 2), dtype=i32), torch.ones(1, dtype=i32), torch.zeros(2, dtype=i32)
+    kv, q = torch.zeros((1, 2, 128), dtype=bf), torch.zeros((1, 4, 128), dtype=bf)
+    w = ops.Weight4(torch.zeros(1024, dtype=u8), torch.zeros(64, dtype=u8), 32, 16, 32)
+    calls = [lambda: ops.kv_append(pool, 0, kv, kv, table, lens, start), lambda: ops.kv_read(pool, 0, table, lens, lens, 1),
+             lambda: ops.kv_attention(q, pool, 0, table, lens, start), lambda: ops.kv_copy_pages(pool, [0], [1]),
+             lambda: ops.kv_set(table, {0: 1}), lambda: ops.linear_w4(torch.zeros((1, 32), dtype=bf), w),
+             lambda: ops.quantize_w4(torch.zeros((32, 16)), 32),
+             lambda: ops.Weight4.from_codes(torch.zeros((32, 16), dtype=u8), torch.zeros((1, 16), dtype=bf))]
+    for call in calls:
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    # one host tensor among device tensors, in each place
+    if torch.cuda.is_available():
+        return
+    try:
+        torch._C._cuda_getDevice()
+    except Exception:
+        real, torch._C._cuda_getDevice = torch._C._cuda_getDevice, lambda: 0
+    else:
+        real = None
+    try:
+        good = [OnDevice(1, 2, 128), OnDevice(1, 2, 128), OnDevice(1, 2, dtype=i32), OnDevice(1, dtype=i32), OnDevice(2, dtype=i32)]
+        pool.k = OnDevice(1, 4, 2, 16, 128, dtype=u8)
+        for i in range(5):
+            args = list(good)
+            args[i] = good[i].t
+            with pytest.raises(ValueError, match="CUDA"):
+                ops.kv_append(pool, 0, *args)
+        with pytest.raises(ValueError, match="current device"):
+            class Elsewhere(OnDevice):
+                def get_device(self):
+                    return 1
+            ops.kv_append(pool, 0, Elsewhere(1, 2, 128), *good[1:])
+    finally:
+        if real is not None:
+            torch._C._cuda_getDevice = real
