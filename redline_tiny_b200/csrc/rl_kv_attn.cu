@@ -65,6 +65,7 @@ struct Args {
   int64_t ldo;
   Div group, hkv;                // query heads per K/V head, K/V heads
   int page_sh;                   // log2 of the page size
+  int vec;                       // rows of o are 8-byte aligned
   float* part;                   // workspace: 2 slots per CTA of R x (128 + 2) floats
   Record* rec;                   // workspace: per CTA, the task it began and did not finish
 };
@@ -152,6 +153,12 @@ __device__ __forceinline__ void unit_prefix(const Args& a, int R, int64_t* pre, 
     for (int w = 0; w < kWarps; ++w) base += warp_sum[w];
     __syncthreads();
   }
+}
+
+// floor(i U / C), in 32 bits where that holds the product.
+__device__ __forceinline__ int64_t share(uint32_t i, int64_t U, int64_t C) {
+  if (U < (1 << 20)) return i * static_cast<uint32_t>(U) / static_cast<uint32_t>(C);   // (a grid has fewer than 2^12 CTAs)
+  return i * U / C;
 }
 
 template <int NT>
@@ -291,6 +298,22 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
   }
 }
 
+// O / l of one row as bf16, 4 dims a lane.
+__device__ __forceinline__ void store_row(const Args& a, int64_t token, uint32_t head, int lane, const float4& o, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* d = a.o + token * a.ldo + head * HD + 4 * lane;
+  const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  if (a.vec) {
+    uint2 w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(v[1]), "f"(v[0]));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(v[3]), "f"(v[2]));
+    *reinterpret_cast<uint2*>(d) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+  }
+}
+
 // Shared memory of a CTA: the ring that brings blocks in (per warp kStages x [K 2 KB | V 2 KB]), reused at the end of a
 // run for the warps' results (kWarps x R x 128 floats), then their maxima and sums, then the unit prefix.
 template <int NT>
@@ -329,8 +352,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
   const int64_t U = pre[a.batch.B];
   const int64_t C = min(static_cast<int64_t>(gridDim.x), U);        // every working CTA has at least one unit
   const bool idle = blockIdx.x >= C;
-  const int64_t u_end = idle ? 0 : (blockIdx.x + 1) * U / C;
-  int64_t u = idle ? 0 : blockIdx.x * U / C;
+  const int64_t u_end = idle ? 0 : share(blockIdx.x + 1, U, C);
+  int64_t u = idle ? 0 : share(blockIdx.x, U, C);
   bool first = true;
   Record rec = {};
   int b = 0;
@@ -387,28 +410,47 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
     lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
 
+    // q of the rows this lane loads: asked for before the copies fill the memory system's queues
+    uint4 qw[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t r = row0 + nt * 8 + g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qw[nt][i] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const uint32_t j = r / a.group;
+        const uint16_t* p = a.q + (s.s0 + j) * a.q_st + (h * a.group.d + r - j * a.group.d) * a.q_sh + 16 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qw[nt][i] = *reinterpret_cast<const uint4*>(p + 64 * (i >> 1) + 8 * (i & 1));
+      }
+    }
+
     // the warp's blocks: every kWarps-th of the run. Lane j holds the pool index of block 32 t + j, one chunk ahead.
     const int64_t key_end = min(ch1 * UNIT, static_cast<int64_t>(lim_max) + 1);
     const int64_t pos0 = ch0 * UNIT + warp * BT;
     const int n = key_end > pos0 ? static_cast<int>((key_end - pos0 + kWarps * BT - 1) / (kWarps * BT)) : 0;
-    auto block_of = [&](int k) -> int {
+    const int32_t* table = a.batch.table + b * a.batch.ld;
+    auto page_of = [&](int k) -> int {                               // (a plain load: nothing waits for it here)
+      return k < n ? __ldg(table + ((static_cast<uint32_t>(pos0) + k * (kWarps * BT)) >> a.page_sh)) : 0;
+    };
+    auto block_in = [&](int pg, int k) -> int {
       if (k >= n) return -1;
-      const uint32_t pos = static_cast<uint32_t>(pos0) + k * (kWarps * BT);
-      const int pg = __ldg(a.batch.table + b * a.batch.ld + (pos >> a.page_sh));
       if (static_cast<uint32_t>(pg) >= a.pool.pages) {               // a page outside the pool: its keys are absent
         report(kErrBadArgument);
         return -1;
       }
+      const uint32_t pos = static_cast<uint32_t>(pos0) + k * (kWarps * BT);
       return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + ((pos & (a.pool.page - 1)) >> 4);
     };
-    int idx = block_of(lane), idx_next = block_of(32 + lane);
+    const int page0 = page_of(lane);
+    int page_next = page_of(32 + lane), idx = block_in(page0, lane);
     uint32_t ke[S], ve[S];                                           // of the ring's blocks
     int at_pos[S];                                                   // first position, or beyond every limit
     auto issue = [&](int k, int j) {
       if (k < n) {
         if ((k & 31) == 0 && k > 0) {
-          idx = idx_next;
-          idx_next = block_of(k + 32 + lane);
+          idx = block_in(page_next, k + lane);
+          page_next = page_of(k + 32 + lane);
         }
         const int found = __shfl_sync(0xffffffffu, idx, k & 31);
         const int64_t blk = max(found, 0);                           // an absent block reads as block 0, fully masked
@@ -431,14 +473,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     // q of the tile, while the first blocks are on their way
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t r = row0 + nt * 8 + g;                          // the row whose q this lane loads
-      uint4 w[4] = {};
-      if (r < rows) {
-        const uint32_t j = r / a.group;
-        const uint16_t* p = a.q + (s.s0 + j) * a.q_st + (h * a.group.d + r - j * a.group.d) * a.q_sh + 16 * c;
-        w[0] = *reinterpret_cast<const uint4*>(p), w[1] = *reinterpret_cast<const uint4*>(p + 8);
-        w[2] = *reinterpret_cast<const uint4*>(p + 64), w[3] = *reinterpret_cast<const uint4*>(p + 72);
-      }
+      const uint4 (&w)[4] = qw[nt];
       const uint32_t x[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
                               w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
       uint32_t mx = 0;
@@ -518,27 +553,28 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     __syncthreads();
     const bool whole = ch0 == 0 && ch1 == nch;
     float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * R * (HD + 2);
-    const int d = threadIdx.x % HD;
-    for (int row = threadIdx.x / HD; row < R; row += kWarps * 32 / HD) {
+    // a warp per row, 4 dims a lane
+#pragma unroll 2
+    for (int row = warp; row < R; row += kWarps) {
       const uint32_t r = row0 + row, j = r / a.group;
       if (r >= rows) break;
-      float m = sm[row];
+      float mw[kWarps], m = kNone;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sm[w * R + row]);
-      float l = 0.0f, o = 0.0f;
+      for (int w = 0; w < kWarps; ++w) mw[w] = sm[w * R + row], m = fmaxf(m, mw[w]);
+      float l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_approx(sm[w * R + row] - m);
-        l += f * sl[w * R + row];
-        o += f * so[(w * R + row) * HD + d];
+        const float f = exp2_approx(mw[w] - m);
+        const float4 v = reinterpret_cast<const float4*>(so + (w * R + row) * HD)[lane];
+        l = fmaf(f, sl[w * R + row], l);
+        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
       }
       if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        a.o[(s.s0 + j) * a.ldo + (h * a.group.d + r - j * a.group.d) * HD + d] =
-            __bfloat16_as_ushort(__float2bfloat16_rn(o * inv));
+        store_row(a, s.s0 + j, h * a.group.d + r - j * a.group.d, lane, o, l);
       } else {
-        part[row * HD + d] = o;
-        if (d == 0) part[R * HD + row] = m, part[R * HD + R + row] = l;
+        reinterpret_cast<float4*>(part + row * HD)[lane] = o;
+        if (lane == 0) part[R * HD + row] = m, part[R * HD + R + row] = l;
       }
     }
     if (!whole && ch0 == 0) {
@@ -624,11 +660,7 @@ __global__ void __launch_bounds__(32 * kJoin) combine_kernel(const Args a) {
         o.z = fmaf(fb, v.z, o.z * fa), o.w = fmaf(fb, v.w, o.w * fa);
       }
       const uint32_t jr = r / a.group;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint16_t* d = a.o + (rec.s0 + jr) * a.ldo + (rec.h * a.group.d + r - jr * a.group.d) * HD + 4 * lane;
-      const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+      store_row(a, rec.s0 + jr, rec.h * a.group.d + r - jr * a.group.d, lane, o, l);
     }
     __syncthreads();
   }

@@ -78,6 +78,7 @@ int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, in
   a.o = o, a.ldo = ldo;
   a.group = kvattn::Div::of(heads / kv_heads), a.hkv = kvattn::Div::of(kv_heads);
   a.page_sh = __builtin_ctz(page);
+  a.vec = aligned(o, 8) && ldo % 4 == 0;
   if (kvattn::by_prompt(T, B, heads, kv_heads, scale_log2)) {
     const kvprompt::Args p{q, q_st, q_sh, a.pool, a.batch, row_limit, scale_log2, o, ldo, a.group, a.hkv, a.page_sh,
                            aligned(o, 16) && ldo % 8 == 0};
