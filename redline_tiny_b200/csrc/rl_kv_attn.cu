@@ -4,8 +4,9 @@
 // With K = 2^(ek-133) mk per block of 16 tokens, s is an fp16 product q~ . mk (mk is an integer in [-128, 127], exact;
 // q~ is q times a power of two per row that puts the row's largest value in [2^14, 2^15), exact for every value within
 // 2^-28 of it) times one fp32 factor per block and row. P is rounded to fp16 (11 significant bits, half a step 2^-11
-// of each weight; the row sum adds them unrounded) and P . mv of a block, again with exact integers, is scaled by
-// 2^(ev-133) as it is added to the fp32 accumulator. So the only roundings are P's and fp32's.
+// of each weight; the row sum adds them unrounded). P . mv, again with exact integers, accumulates in fp32 in units of
+// 2^(er-133), er the largest V exponent so far; a block's own scale 2^(ev-er) goes into its P. So the only roundings are
+// P's and fp32's.
 //
 // The rows of one K/V head that share its keys (tokens of a sequence x query heads of the group) are the N side of
 // mma.m16n8k16: S^T (16 tokens x 8 rows) = K q~^T and O^T (16 dims x 8 rows) += V^T P^T. The cache is then the A
@@ -17,6 +18,11 @@
 // Work is split evenly over the CTAs whatever the lengths are: a task is (sequence, K/V head, 8 NT rows), its units
 // are 64 keys; CTA i takes units [i U / C, (i + 1) U / C) of the whole list. A task that a CTA does not finish leaves
 // (O, m, l) in the workspace, and combine_kernel joins the pieces in CTA order, so results do not depend on timing.
+//
+// Bound by the cache's bytes for one token a sequence: 269 MB (one sequence of 131071 tokens, 8 heads) in 54 us, of which
+// the loop over the keys takes 35 - 46 us a CTA (7.6 - 5.8 TB/s), its start 4 and the joins 5; 564 MB (64 sequences of up
+// to 8192) in 100 us = 5.7 TB/s. A step of 777 keys takes 7.0 us: two launches and four memory latencies. Steps, for the
+// two: plain loads 114 / 166 us; copies through a per-warp ring 67 / 114; V scales in P and no 64-bit divisions 55 / 102.
 #include "rl_common.cuh"
 #include "rl_host.h"
 

@@ -10,12 +10,16 @@
 //    2^(ek - 133) is applied to S, 16 columns at a time, where the softmax scales them anyway. V: fp16 (u - 128) 2^(ev - e),
 //    exact down to 2^-24, with e the largest V exponent that the tile sees, found before the first block; O is multiplied by
 //    2^(e - 133) at the end. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
-//    same layout read as MN-major B.
+//    same layout read as MN-major B. The codes wait in the converters' registers for the time of a block (with one item in
+//    flight their latency bound the kernel: 791 us for the case below, staged through shared memory 346).
 //  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
 //  * the tile's rows need not be consecutive in memory, so Q is copied by the converter warps as well.
 //
-// 3300 cycles per block of the two tiles, as the dense kernel: the softmax's exponentials and the MMAs bound it, the
-// converters (310 instructions a lane and block) fit beside them.
+// The softmax and its MMAs bound it: 4850 cycles per block of both tiles (3000 of them the softmax's, which shares the
+// issue slots and the shared memory with the converters; the dense kernel takes 3300 in all), the converters work 3300.
+// Three prompt chunks of 1021, 650 and 279 tokens over 8191, 5214 and 2245 (32 heads over 8): 267 us, 713 TFLOP/s; a fifth
+// of it is the tail of 256 tiles of three lengths on 148 SMs. Rejected: reading S twice to free registers (361 - 424 us),
+// the scales read from shared memory where they are used (280 us).
 #include "rl_common.cuh"
 #include "rl_host.h"
 
@@ -123,9 +127,11 @@ __device__ __forceinline__ void write_unit(uint8_t* tile, int r0, const Unit& u,
 }
 
 // One 128-key block of the online softmax of the thread's row, as rl_attn.cu's softmax_block with a scale per 16 keys.
-__device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0, int lim, const float* scale,
+__device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0, int lim, const float* scale_at,
                                               uint2 flags, bool o_live, float& m_run, float& l_run, uint64_t* p_bar,
                                               int lane) {
+  const float4 sa = *reinterpret_cast<const float4*>(scale_at), sb = *reinterpret_cast<const float4*>(scale_at + 4);
+  const float scale[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
   uint32_t s[BKV];
 #pragma unroll
   for (int c = 0; c < BKV / 32; ++c) {
