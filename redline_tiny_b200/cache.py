@@ -22,6 +22,12 @@ import torch
 from . import ops
 
 
+def _not_captured(what):
+    """The books move on the host when the call is made, not when a captured graph is replayed."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} keeps books on the host and cannot be captured into a graph")
+
+
 class OutOfPages(RuntimeError):
     """The pool has fewer free pages than a step needs; nothing was changed."""
 
@@ -35,6 +41,7 @@ class PagedKV:
         self._seqs = {}                    # sequence -> its pages in order
         self._len = {}
         self._next = 0
+        self._version = 0                  # grows when pages move: a batch's tables are then out of date
 
     # -- books ------------------------------------------------------------------------------------------------------
     def new(self):
@@ -125,6 +132,7 @@ class PagedKV:
     def compact(self):
         """Move the live pages to the front of the pool, so that its tail can be given back (resize). Returns the number
         of pages moved. A batch follows at its next `extend` (of no tokens, if need be), not before."""
+        _not_captured("compact")
         live = [p for p, r in enumerate(self.refs) if r]
         n = len(live)
         to = dict(zip([p for p in live if p >= n], [p for p in range(n) if not self.refs[p]]))
@@ -135,10 +143,12 @@ class PagedKV:
             for pages in self._seqs.values():
                 pages[:] = [to.get(p, p) for p in pages]
             self._free = list(range(n, len(self.refs)))
+            self._version += 1
         return len(to)
 
     def resize(self, pages):
         """A pool of `pages` pages (compacted first when that drops any). Captured graphs hold the old one."""
+        _not_captured("resize")
         if pages < len(self.refs):
             if pages < sum(1 for r in self.refs if r):
                 raise OutOfPages(f"{sum(1 for r in self.refs if r)} pages are in use")
@@ -167,18 +177,26 @@ class Batch:
         self._meta = torch.full((B * self.width + 2 * B + 1,), -1, dtype=torch.int32, device=dev)
         self._meta[B * self.width:] = 0
         self._written = [[] for _ in self.seqs]      # what the device tables hold
-        self._lens, self._starts = [0] * B, [0] * (B + 1)
+        self._lens, self._starts, self._version = [0] * B, [0] * (B + 1), kv._version
         self.table = self._meta[:B * self.width].view(B, self.width)
         self.kv_len = self._meta[B * self.width:B * self.width + B]
         self.q_start = self._meta[B * self.width + B:]
 
     @property
     def args(self):
+        if self._version != self.kv._version:
+            raise RuntimeError("the cache's pages have moved since this batch's last extend")
         return self.table, self.kv_len, self.q_start
+
+    @property
+    def rows(self):
+        """New tokens of the last extend."""
+        return self._starts[-1]
 
     def extend(self, counts):
         """Make room for counts[i] new tokens of each sequence and point the device arrays at them: pages are taken,
         shared pages that will be written are copied. Raises OutOfPages, with nothing changed, where the pool is full."""
+        _not_captured("extend")
         counts = list(counts)
         kv, B = self.kv, len(self.seqs)
         if len(counts) != B:
@@ -209,5 +227,6 @@ class Batch:
             if self._starts[b] != at:
                 self._starts[b] = new[B * W + B + b] = at
             at += counts[b] if b < B else 0
+        self._version = kv._version
         if new:
             ops.kv_set(self._meta, new)

@@ -438,8 +438,8 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     """Attention of new tokens q (T, heads, 128) bf16 (any row and head strides that are multiples of 8) over a layer of
     the cache, which holds their own keys already (kv_append). Row j of sequence b's n new rows sees positions
     <= kv_len[b] - n + j, or <= min(row_limit[row], kv_len[b] - 1) with row_limit int32 (T); a row that sees no key gives
-    zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128). scale_log2 defaults to
-    log2(e)/sqrt(128)."""
+    zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128); `out` must not overlap q. scale_log2
+    defaults to log2(e)/sqrt(128)."""
     dev = _here(q, pool.k, table, kv_len, q_start, row_limit, out)
     B, width = _batch(table, kv_len, q_start, 1)
     if q.dim() != 3 or q.dtype is not torch.bfloat16:
@@ -454,10 +454,15 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
         out = q.new_empty((T, H * 128))
     elif out.dtype is not torch.bfloat16 or out.shape != (T, H * 128) or out.stride(1) != 1:
         raise ValueError(f"out must be bf16 ({T}, {H * 128}) with contiguous rows")
+    if T == 1:
+        st = 0   # a single row's stride says nothing
+    if H == 1:
+        sh = 0
+    ldo = H * 128 if T == 1 else out.stride(0)
     ws = pool.k.new_empty(_kv_attention_workspace(dev, T, B, H, pool.kv_heads))
     L.call("rl_kv_attention", q.data_ptr(), st, sh, T, H, *pool._args(layer), table.data_ptr(), width,
            kv_len.data_ptr(), q_start.data_ptr(), B, None if row_limit is None else row_limit.data_ptr(),
-           _SCALE_LOG2 if scale_log2 is None else scale_log2, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+           _SCALE_LOG2 if scale_log2 is None else scale_log2, out.data_ptr(), ldo, ws.data_ptr(), ws.numel(),
            _stream_of(dev))
     return out
 
@@ -528,7 +533,7 @@ def _w4(x, w, bias, epi, out, cols, out_dtype):
 
 def linear_w4(x, w, bias=None, out=None, out_dtype=torch.bfloat16):
     """C = x @ B (+ bias) for up to 64 rows x (M, K) bf16 (any bf16 values) and a Weight4: the products of a decode step
-    (linear_bfp16 takes more rows)."""
+    (linear_bfp16 takes more rows). `out` must not overlap x."""
     if w.swiglu:
         raise ValueError("linear_w4 takes a Weight4 packed without swiglu (swiglu_w4 takes the others)")
     return _w4(x, w, bias, L.RL_EPI_NONE if bias is None else L.RL_EPI_BIAS, out, w.N, out_dtype)

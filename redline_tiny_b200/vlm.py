@@ -186,6 +186,9 @@ class CachedLM:
         (T, 64): the RoPE rows of their positions. Appends their keys and values to every layer's cache and returns the
         residual stream after the last layer, bf16 (T, hidden)."""
         cfg, T = self.cfg, x.shape[0]
+        if batch.kv is not self.kv or T != batch.rows:
+            raise ValueError(f"{T} rows for a batch with {batch.rows} new tokens" if batch.kv is self.kv else
+                             "the batch belongs to another cache")
         if T == 0:
             return x
         rope = torch.stack([cos.float(), sin.float()], -1).reshape(T, 128).contiguous()

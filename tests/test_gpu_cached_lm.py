@@ -160,3 +160,45 @@ def test_two_streams_and_two_graphs(env):
     ops.device_status()
     for i in range(2):
         assert torch.equal(outs[i], alone[i])
+
+
+def test_refusals(env):
+    torch, ops, vlm, cache, dev = env
+    cfg = vlm.LMConfig(hidden=256, heads=2, kv_heads=1, ffn=256, layers=1)
+    kv = cache.PagedKV(1, 8, 1, 16)
+    lm = vlm.CachedLM(cfg, vlm.random_lm_weights(cfg), kv, few=8)
+    batch = kv.batch([kv.new()])
+    batch.extend([3])
+    x, rope = torch.zeros((2, 256), dtype=torch.bfloat16, device=dev), torch.zeros((2, 64), device=dev)
+    with pytest.raises(ValueError, match="2 rows"):
+        lm.forward(x, batch, rope, rope)
+    other = cache.PagedKV(1, 8, 1, 16)
+    step = other.batch([other.new()])
+    step.extend([2])
+    with pytest.raises(ValueError, match="another cache"):
+        lm.forward(x, step, rope, rope)
+    with pytest.raises(ValueError, match="layers"):
+        vlm.CachedLM(vlm.LMConfig(hidden=256, heads=2, kv_heads=2, ffn=256), {"layers": []}, kv)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=dev)
+        for call in (lambda: batch.extend([1]), kv.compact, lambda: kv.resize(4)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+
+
+def test_one_row_views_with_odd_strides(env):
+    """A single row or head, whose stride says nothing, is taken with any stride."""
+    torch, ops, vlm, cache, dev = env
+    kv = cache.PagedKV(1, 8, 1, 16)
+    batch = kv.batch([kv.new()])
+    batch.extend([1])
+    g = torch.Generator(device=dev)
+    g.manual_seed(1)
+    x = torch.randn((1, 1, 128), generator=g, device=dev).to(torch.bfloat16)
+    ops.kv_append(kv.pool, 0, x, x, *batch.args)
+    want = ops.kv_attention(x, kv.pool, 0, *batch.args)
+    odd = torch.as_strided(x, (1, 1, 128), (3, 5, 1))
+    out = torch.as_strided(torch.zeros(256, dtype=torch.bfloat16, device=dev), (1, 128), (7, 1))
+    assert torch.equal(ops.kv_attention(odd, kv.pool, 0, *batch.args, out=out), want)
+    ops.device_status()

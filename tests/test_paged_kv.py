@@ -168,3 +168,22 @@ def test_refusals(fake):
         batch.extend([1, 1])
     with pytest.raises(cache.OutOfPages, match="in use"):
         kv.resize(0)
+
+
+def test_a_compacted_cache_asks_for_an_extend(fake):
+    """Page tables written before pages moved are not handed out."""
+    kv = cache.PagedKV(1, 8, 1, PAGE, "cpu")
+    a, b = kv.new(), kv.new()
+    batch = kv.batch([a, b])
+    batch.extend([PAGE, 2 * PAGE])
+    assert batch.rows == 3 * PAGE
+    only = kv.batch([b])
+    only.extend([1])
+    kv.free(a)
+    assert kv.compact() == 1
+    with pytest.raises(RuntimeError, match="moved"):
+        only.args
+    only.extend([0])
+    assert only.table[0, :3].tolist() == list(kv.pages(b)) and sorted(kv.pages(b)) == [0, 1, 2]
+    assert only.rows == 0 and kv.compact() == 0
+    only.args
