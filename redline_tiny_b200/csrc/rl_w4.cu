@@ -1,9 +1,12 @@
 // Products of a few rows with 4-bit weights: C[m][n] = sum_k x[m][k] (u[n][k] - 8) s[n][k / G] (+ bias), m < 64.
 //
-// Bound by the weight bytes (K N / 2) at one row, by instruction issue from there on. The weights are the A operand of
+// Bound by the weight bytes (K N / 2) on paper at one row; what the kernels reach is set by the half-rate ALU pipe and the
+// latency of short streams: 50 MB of codes (4096 x 24576, one row) take 13.9 us = 3.8 TB/s with the ALU pipe at 44 % and
+// issue at 50 %, 12.6 MB (4096 x 6144) 4.6 - 5 us, of which a launch and one load are 4. The weights are the A operand of
 // mma.m16n8k16 (16 columns of B on the M side, up to 8 rows of x per n-tile), turned from 4 bits to bf16 in registers,
 // exactly (nibbles_lo). A group's products are summed by the tensor core in fp32 and scaled once as they are added to the
-// fp32 result, so the only rounding is the output's (and fp32's).
+// fp32 result, so the only rounding is the output's (and fp32's). Rejected for one row: two column tiles a warp (17.4 us),
+// 2 - 4 warps a CTA (16.8 - 18.4), CTAs that go on to further columns (15.2), deeper rings (no change).
 //
 // Native layout, 0.5 byte a weight: tiles of 16 columns x 128 k, 1 KB, K running fastest. Lane 4g + c owns 16 bytes for
 // column g (first 512 bytes) and 16 for column g + 8; word q of them holds k = 32q + 8c .. + 7, nibble i the k 2i and
@@ -260,7 +263,9 @@ __global__ void __launch_bounds__(32 * kFew, 4) few_kernel(const Args a) {
 // 9 to 64 rows: one CTA per 128 columns and share of K, a warp per CT x 16 columns; the x of a share is brought into
 // shared memory once (with one warp per 16 columns reading x itself, x is M / 8 times the weights' bytes of L2 traffic)
 // and each fragment serves CT tiles of codes. The CTAs of a cluster hold the shares of K of the same columns and are
-// joined through distributed shared memory in rank order.
+// joined through distributed shared memory in rank order. 23 rows, 12288 x 4096: 14.3 us. mma.sync issues one m16n8k16 in
+// two cycles an SM (1024 products a cycle): 24 of them a tile and 192 tiles on the fullest SMs are 5 us, start, joins and
+// clusters that leave SMs empty the rest; 64 rows reach 200 - 226 TFLOP/s. Rejected: K split over warps as well (17 - 19 us).
 template <int NT>
 struct Many {
   static constexpr int CT = NT <= 3 ? 2 : 1;
