@@ -120,6 +120,12 @@ def call(name, *args):
     return st
 
 
+def check(name, st):
+    """Raise RedlineError for a non-zero status of a call made elsewhere on this thread."""
+    if st != RL_OK:
+        raise RedlineError(name, st, lib().rl_last_error().decode(errors="replace"))
+
+
 def device_status():
     """Synchronise and read / clear the device error word; raises on a device-side error."""
     flags = ctypes.c_int(0)

@@ -1,4 +1,5 @@
-"""Build libredline_b200.so in-tree with nvcc for sm_100a (no GPU needed: nvcc cross-compiles).
+"""Build libredline_b200.so in-tree with nvcc for sm_100a (no GPU needed: nvcc cross-compiles), and the Python extension
+_rl_torch.so (the hot calls of ops.py in C++) beside it.
 
     python -m redline_tiny_b200.build [--verbose]
 """
@@ -15,30 +16,55 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a",
               "-Xcompiler", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include")]
 
 
+EXT_SRC = os.path.join(HERE, "csrc", "rl_torch.cpp")
+EXT = os.path.join(HERE, "_rl_torch.so")
+HEADER = os.path.join(ROOT, "include", "redline_b200.h")
+
+
 def sources():
     d = os.path.join(HERE, "csrc")
-    return [os.path.join(d, f) for f in sorted(os.listdir(d))] + [os.path.join(ROOT, "include", "redline_b200.h")]
+    return [os.path.join(d, f) for f in sorted(os.listdir(d)) if f != "rl_torch.cpp"] + [HEADER]
 
 
-def up_to_date():
-    if not os.path.exists(OUT):
+def up_to_date(out=OUT, srcs=None):
+    if not os.path.exists(out):
         return False
-    t = os.path.getmtime(OUT)
-    return all(os.path.getmtime(s) <= t for s in sources())
+    t = os.path.getmtime(out)
+    return all(os.path.getmtime(s) <= t for s in srcs or sources())
 
 
-def build(verbose=False, force=False):
-    if not force and up_to_date():
-        return OUT
-    nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", OUT + ".tmp", SRC]
+def build_extension(verbose=False, force=False):
+    if not force and up_to_date(EXT, [EXT_SRC, HEADER]):
+        return EXT
+    import sysconfig
+
+    import torch
+    t = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-o", EXT + ".tmp", EXT_SRC,
+          "-I", sysconfig.get_paths()["include"], "-isystem", f"{t}/include", "-isystem",
+          f"{t}/include/torch/csrc/api/include", "-isystem", f"{cuda}/include",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-L", HERE, "-l:libredline_b200.so", "-L",
+          f"{t}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
+    os.replace(EXT + ".tmp", EXT)
+    return EXT
+
+
+def _run(cmd, verbose):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError(f"nvcc failed ({r.returncode}): {' '.join(cmd)}")
+        raise RuntimeError(f"{cmd[0]} failed ({r.returncode}): {' '.join(cmd)}")
     if verbose:
         sys.stderr.write(r.stdout + r.stderr)
-    os.replace(OUT + ".tmp", OUT)
+
+
+def build(verbose=False, force=False):
+    if force or not up_to_date():
+        nvcc = os.environ.get("NVCC", "nvcc")
+        _run([nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", OUT + ".tmp", SRC], verbose)
+        os.replace(OUT + ".tmp", OUT)
+    build_extension(verbose, force)
     return OUT
 
 

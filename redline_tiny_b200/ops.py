@@ -25,6 +25,11 @@ import torch
 
 from . import _lib as L
 
+try:   # the hot calls in one step each (csrc/rl_torch.cpp); None: through ctypes, with the same checks and results
+    from . import _rl_torch as _fast
+except ImportError:
+    _fast = None
+
 
 def _stream():
     return ctypes_ptr(torch.cuda.current_stream().cuda_stream)
@@ -342,6 +347,8 @@ class KVPool:
     (layers, pages, kv_heads, page / 16). A block of 16 tokens of one head shares one exponent:
     value = (k - 128) * 2^(k_exp - 133); exponent 255 reads as NaN."""
 
+    _fast = ()   # per layer: what _rl_torch takes for it
+
     def __init__(self, k, v, k_exp, v_exp):
         _here(k, v, k_exp, v_exp)
         if k.dim() != 5 or k.shape[4] != 128 or k.shape[3] not in (16, 32, 64, 128, 256):
@@ -353,6 +360,7 @@ class KVPool:
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.layers, self.pages, self.kv_heads, self.page = k.shape[:4]
         self._ptrs = [tuple(t[i].data_ptr() for t in (k, v, k_exp, v_exp)) for i in range(self.layers)]
+        self._fast = [(*self._args(i), k.get_device()) for i in range(self.layers)]
 
     @classmethod
     def empty(cls, layers, pages, kv_heads, page=64, device="cuda"):
@@ -387,6 +395,10 @@ def kv_append(pool, layer, k, v, table, kv_len, q_start):
     cache. table int32 (B, pages), kv_len int32 (B) with the new tokens counted, q_start int32 (B + 1): the new tokens
     of sequence b are rows q_start[b] .. q_start[b + 1] - 1 and take its last positions. A block's exponent grows to
     hold them, and older codes of the block are shifted. The pages written must belong to one sequence each."""
+    if _fast is not None and 0 <= layer < len(pool._fast):
+        st = _fast.kv_append(pool._fast[layer], k, v, table, kv_len, q_start)
+        if st is not None:
+            return L.check("rl_kv_append", st)
     dev = _here(pool.k, k, v, table, kv_len, q_start)
     B, width = _batch(table, kv_len, q_start, 1)
     T = k.shape[0]
@@ -399,6 +411,10 @@ def kv_append(pool, layer, k, v, table, kv_len, q_start):
 def kv_read(pool, layer, table, kv_len, start, count):
     """Positions start[b] .. start[b] + count - 1 of each sequence of a layer as (k, v) bf16 (B, count, kv_heads, 128),
     exactly; zeros at and after kv_len[b]."""
+    if _fast is not None and 0 <= layer < len(pool._fast):
+        out = _fast.kv_read(pool._fast[layer], table, kv_len, start, count)
+        if out is not None:
+            return out if type(out) is tuple else L.check("rl_kv_read", out)
     dev = _here(pool.k, table, kv_len, start)
     B, width = _batch(table, kv_len, start, 0)
     kv = torch.empty((2, B, count, pool.kv_heads, 128), dtype=torch.bfloat16, device=pool.k.device)
@@ -440,6 +456,11 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     <= kv_len[b] - n + j, or <= min(row_limit[row], kv_len[b] - 1) with row_limit int32 (T); a row that sees no key gives
     zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128); `out` must not overlap q. scale_log2
     defaults to log2(e)/sqrt(128)."""
+    scale = _SCALE_LOG2 if scale_log2 is None else float(scale_log2)
+    if _fast is not None and 0 <= layer < len(pool._fast):
+        o = _fast.kv_attention(q, pool._fast[layer], table, kv_len, q_start, row_limit, scale, out)
+        if o is not None:
+            return o if type(o) is not int else L.check("rl_kv_attention", o)
     dev = _here(q, pool.k, table, kv_len, q_start, row_limit, out)
     B, width = _batch(table, kv_len, q_start, 1)
     if q.dim() != 3 or q.dtype is not torch.bfloat16:
@@ -462,7 +483,7 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     ws = pool.k.new_empty(_kv_attention_workspace(dev, T, B, H, pool.kv_heads))
     L.call("rl_kv_attention", q.data_ptr(), st, sh, T, H, *pool._args(layer), table.data_ptr(), width,
            kv_len.data_ptr(), q_start.data_ptr(), B, None if row_limit is None else row_limit.data_ptr(),
-           _SCALE_LOG2 if scale_log2 is None else scale_log2, out.data_ptr(), ldo, ws.data_ptr(), ws.numel(),
+           scale, out.data_ptr(), ldo, ws.data_ptr(), ws.numel(),
            _stream_of(dev))
     return out
 
@@ -478,6 +499,7 @@ class Weight4:
         self.codes, self.scales = codes, scales
         self.K, self.N, self.group, self.swiglu = int(K), int(N), int(group), bool(swiglu)
         self._ptrs = codes.data_ptr(), scales.data_ptr()
+        self._fast = (*self._ptrs, self.K, self.N, self.group, codes.get_device())
 
     @classmethod
     def from_codes(cls, codes, scales, swiglu=False):
@@ -514,6 +536,10 @@ def quantize_w4(B, group=64):
 
 
 def _w4(x, w, bias, epi, out, cols, out_dtype):
+    if _fast is not None and out is None and (out_dtype is torch.bfloat16 or out_dtype is torch.float32):
+        o = _fast.linear_w4(x, w._fast, bias, epi, cols, out_dtype is torch.float32)
+        if o is not None:
+            return o if type(o) is not int else L.check("rl_linear_w4", o)
     dev = _here(x, w.codes, bias, out)
     M = x.shape[0]
     if x.shape != (M, w.K) or x.dtype is not torch.bfloat16:

@@ -372,3 +372,107 @@ def test_append_and_attend_in_a_graph(env, path):
         ops.device_status()
         same_pool(c)
         check_attention(out, *c.oracle(d[2]))
+
+
+def test_both_bindings(env, monkeypatch):
+    """The compiled binding and the ctypes one write, read, attend and refuse alike, whatever strides and optional
+    arguments they are given."""
+    torch, ops, L, dev = env
+    assert ops._fast is not None, "the extension is built with the library"
+    results = []
+    for binding in (ops._fast, None):
+        monkeypatch.setattr(ops, "_fast", binding)
+        c = Case(torch, ops, dev, [90, 33, 40], [20, 0, 3], 2, 16, seed=21)
+        x = O.bf16_round(c.rng.standard_normal((c.T, 2, 128)).astype(np.float32))
+        q = O.bf16_round(c.rng.standard_normal((c.T, 4, 128)).astype(np.float32))
+        k, qt = bf16(torch, x, dev), bf16(torch, q, dev)
+        kt = k.transpose(0, 1).contiguous().transpose(0, 1)
+        ops.kv_append(c.pool, 0, kt, k, *c.args()[2:])
+        ops.kv_append(c.pool, 0, kt.float(), k.float(), *c.args()[2:])
+        got = [c.pool.k, c.pool.v, c.pool.k_exp, *ops.kv_read(c.pool, 0, c.d_table, c.d_len, c.d_len - 30, 35)]
+        lim = torch.arange(c.T, dtype=torch.int32, device=dev)
+        out = torch.zeros((c.T, 1024), dtype=torch.bfloat16, device=dev)
+        got += [ops.kv_attention(qt, *c.args()), ops.kv_attention(qt, *c.args(), row_limit=lim, scale_log2=0.1),
+                ops.kv_attention(qt[:, ::2], c.pool, 0, *c.args()[2:]), ops.kv_attention(qt, *c.args(), out=out[:, 512:]), out]
+        w = ops.Weight4.from_float(torch.arange(64 * 48, device=dev).reshape(64, 48).float().cos(), 32)
+        b = torch.ones(48, dtype=torch.bfloat16, device=dev)
+        xs = k.reshape(-1, 64)[:5].contiguous()
+        got += [ops.linear_w4(xs, w), ops.linear_w4(xs, w, bias=b), ops.linear_w4(xs, w, out_dtype=torch.float32),
+                ops.linear_w4(xs, w, out=torch.empty((5, 48), device=dev))]
+        for bad in (lambda: ops.kv_attention(qt.float(), *c.args()), lambda: ops.kv_append(c.pool, 0, kt[:, :1], k[:, :1], *c.args()[2:]),
+                    lambda: ops.kv_attention(qt, c.pool, 1, *c.args()[2:]), lambda: ops.kv_attention(qt, c.pool, -1, *c.args()[2:]),
+                    lambda: ops.kv_read(c.pool, 0, c.d_table, c.d_len.long(), c.d_len, 3), lambda: ops.linear_w4(xs.t(), w),
+                    lambda: ops.linear_w4(xs.cpu(), w), lambda: ops.kv_attention(qt.cpu(), *c.args()),
+                    lambda: ops.linear_w4(xs, w, bias=b[:40])):
+            with pytest.raises(ValueError):
+                bad()
+        with pytest.raises(L.RedlineError, match="heads"):
+            ops.kv_attention(qt[:, :3], *c.args())
+        with pytest.raises(L.RedlineError, match="rows"):
+            ops.linear_w4(torch.zeros((65, 64), dtype=torch.bfloat16, device=dev), w)
+        ops.device_status()
+        results.append([t.clone() for t in got])
+    for a, b in zip(*results):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_pages_behind_four_gigabytes(env, path):
+    """Writes, reads, copies and attention at byte offsets that pass 32 bits (codes of K and of V: 4.8 GB each)."""
+    torch, ops, L, dev = env
+    pages, hkv, page = 36500, 8, 128
+    pool = ops.KVPool.empty(1, pages, hkv, page)
+    rng = np.random.default_rng(31)
+    kv = 300
+    table = np.array([[pages - 1, 3, pages - 7]], np.int32)
+    d_table, d_len = torch.from_numpy(table).to(dev), torch.tensor([kv], dtype=torch.int32, device=dev)
+    start = torch.tensor([0, kv], dtype=torch.int32, device=dev)
+    x = [O.bf16_round(rng.standard_normal((kv, hkv, 128)).astype(np.float32)) for _ in range(2)]
+    ops.kv_append(pool, 0, *(bf16(torch, a, dev) for a in x), d_table, d_len, start)
+    kr, vr = ops.kv_read(pool, 0, d_table, d_len, torch.zeros(1, dtype=torch.int32, device=dev), kv)
+    # the same sequence in a small pool
+    small = ops.KVPool.empty(1, 4, hkv, page)
+    t2 = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=dev)
+    ops.kv_append(small, 0, *(bf16(torch, a, dev) for a in x), t2, d_len, start)
+    ks, vs = ops.kv_read(small, 0, t2, d_len, torch.zeros(1, dtype=torch.int32, device=dev), kv)
+    assert torch.equal(kr, ks) and torch.equal(vr, vs)
+    q = bf16(torch, rng.standard_normal((5, 16, 128)).astype(np.float32), dev)
+    rows = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    want = ops.kv_attention(q, small, 0, t2, d_len, rows)
+    assert torch.equal(ops.kv_attention(q, pool, 0, d_table, d_len, rows), want)
+    ops.kv_copy_pages(pool, [pages - 1, 3, pages - 7], [11, pages - 20, 12])
+    t3 = torch.tensor([[11, pages - 20, 12]], dtype=torch.int32, device=dev)
+    assert torch.equal(ops.kv_attention(q, pool, 0, t3, d_len, rows), want)
+    ops.device_status()
+
+
+def test_the_kernel_goes_by_shape(env):
+    """A decode step takes the split kernel and a long chunk the prompt kernel; they agree within two weights' rounding and
+    the output's."""
+    torch, ops, L, dev = env
+    for kv, new, H, hkv, which in (([500, 300], [1, 1], 8, 2, 1), ([900, 700], [900, 700], 32, 8, 2)):
+        c = Case(torch, ops, dev, kv, new, hkv, 64, seed=41)
+        q = bf16(torch, c.rng.standard_normal((c.T, H, 128)).astype(np.float32), dev)
+        got = []
+        for path in (0, 1, 2):
+            before = ops.set_kv_attention_path(path)
+            got.append(ops.kv_attention(q, *c.args()))
+            ops.set_kv_attention_path(before)
+        ops.device_status()
+        assert torch.equal(got[0], got[which])
+        a, b = got[1].float(), got[2].float()
+        top = b.abs().reshape(c.T, H, 128).amax(-1, keepdim=True).expand(-1, -1, 128).reshape_as(b)
+        assert ((a - b).abs() <= 2.0 ** -7 * top).all()
+
+
+def test_steps_with_many_sequences(env):
+    """1024 sequences of up to 40 tokens, the most a call takes; one more is refused."""
+    torch, ops, L, dev = env
+    kv = [1 + i % 40 for i in range(1024)]
+    c = Case(torch, ops, dev, kv, [1] * 1024, 1, 16, seed=51)
+    q = O.bf16_round(c.rng.standard_normal((c.T, 2, 128)).astype(np.float32))
+    got = ops.kv_attention(bf16(torch, q, dev), *c.args())
+    ops.device_status()
+    check_attention(got, *c.oracle(q))
+    t = torch.zeros((1025, 1), dtype=torch.int32, device=dev)
+    with pytest.raises(L.RedlineError, match="1025 sequences"):
+        ops.kv_attention(bf16(torch, q, dev), c.pool, 0, t, t[:, 0].contiguous(), torch.zeros(1026, dtype=torch.int32, device=dev))
