@@ -440,7 +440,7 @@ int rl_kv_set(int32_t* dst, int64_t size, const int32_t* at, const int32_t* valu
  */
 size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads);
 /* Kernel choice, for tests and measurements: 0 = by shape, 1 = the split kernel, 2 = the prompt kernel (positive scales
- * only). Returns the previous choice. */
+ * only), 3 = the split kernel's one-launch form. Returns the previous choice. */
 int rl_set_kv_attention_path(int path);
 int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, int heads, const uint8_t* pool_k,
                     const uint8_t* pool_v, const uint8_t* pool_ke, const uint8_t* pool_ve, int64_t pages, int kv_heads,

@@ -21,8 +21,9 @@
 //
 // Bound by the cache's bytes for one token a sequence: 269 MB (one sequence of 131071 tokens, 8 heads) in 54 us, of which
 // the loop over the keys takes 35 - 46 us a CTA (7.6 - 5.8 TB/s), its start 4 and the joins 5; 564 MB (64 sequences of up
-// to 8192) in 100 us = 5.7 TB/s. A step of 777 keys takes 7.0 us: two launches and four memory latencies. Steps, for the
-// two: plain loads 114 / 166 us; copies through a per-warp ring 67 / 114; V scales in P and no 64-bit divisions 55 / 102.
+// to 8192) in 100 us = 5.7 TB/s. Steps, for the two: plain loads 114 / 166 us; copies through a per-warp ring 67 / 114; V
+// scales in P and no 64-bit divisions 55 / 102. A step of 777 keys takes 5.5 us in one launch of clusters (7.0 in two
+// launches): the launch, three dependent loads, a block or two a warp, the joins.
 #include "rl_common.cuh"
 #include "rl_host.h"
 
@@ -131,8 +132,8 @@ __device__ __forceinline__ int64_t tiles_of(const Args& a, const kv::Seq& s, int
 }
 __device__ __forceinline__ int64_t chunks_of(const kv::Seq& s) { return s.len > 0 ? (s.len + UNIT - 1) / UNIT : 1; }
 
-// Prefix sums of the sequences' units into `pre` (B + 1 values), by the whole CTA.
-template <int kWarps>
+// Prefix sums of the sequences' units (kTasks: of their tasks) into `pre` (B + 1 values), by the whole CTA.
+template <int kWarps, bool kTasks>
 __device__ __forceinline__ void unit_prefix(const Args& a, int R, int64_t* pre, int64_t* warp_sum, int4* seqs) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) pre[0] = 0;
@@ -143,7 +144,7 @@ __device__ __forceinline__ void unit_prefix(const Args& a, int R, int64_t* pre, 
     if (b < a.batch.B) {
       const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
       seqs[b] = make_int4(static_cast<int>(s.s0), static_cast<int>(s.n), static_cast<int>(s.len), 0);
-      if (s.ok) u = tiles_of(a, s, R) * chunks_of(s) * a.hkv.d;
+      if (s.ok) u = tiles_of(a, s, R) * (kTasks ? 1 : chunks_of(s)) * a.hkv.d;
       else if (blockIdx.x == 0) report(kErrBadArgument);
     }
 #pragma unroll
@@ -334,12 +335,27 @@ struct Cfg {
   static constexpr int kStages = NT == 1 ? 3 : 5;
   static constexpr int kRing = kWarps * kStages * 2 * BT * HD;
   static constexpr int kOut = kWarps * R * HD * 4;
-  static constexpr int kBody = kRing > kOut ? kRing : kOut;
+  static constexpr int kJoined = R * (HD + 2) * 4;                    // the CTA's own piece, for its cluster
+  static constexpr int kBody = kRing > kOut + kJoined ? kRing : kOut + kJoined;
   static constexpr int kQ = NT == 1 ? 0 : NT * 16 * 32 * 4;            // q fragments, where registers cannot hold them
   static size_t smem(int B) { return kBody + kQ + kWarps * R * 8 + B * 16 + (kWarps + B + 1) * 8; }
 };
 
-template <int NT>
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float ld_cluster1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// kCluster: short contexts in one launch. A task is one cluster of eight CTAs, which share its keys evenly and join their
+// pieces through distributed shared memory; otherwise units are spread over the grid and combine_kernel joins the pieces.
+constexpr int kClusterCtas = 8;
+template <int NT, bool kCluster>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kernel(const Args a) {
   constexpr int R = 8 * NT, kWarps = Cfg<NT>::kWarps;
   constexpr int S = Cfg<NT>::kStages;
@@ -353,13 +369,20 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
   int64_t* pre = warp_sum + kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  unit_prefix<kWarps>(a, R, pre, warp_sum, seqs);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  unit_prefix<kWarps, kCluster>(a, R, pre, warp_sum, seqs);
   const int64_t U = pre[a.batch.B];
-  const int64_t C = min(static_cast<int64_t>(gridDim.x), U);        // every working CTA has at least one unit
-  const bool idle = blockIdx.x >= C;
-  const int64_t u_end = idle ? 0 : share(blockIdx.x + 1, U, C);
-  int64_t u = idle ? 0 : share(blockIdx.x, U, C);
+  int64_t C = 1, u, u_end;
+  const int rank = blockIdx.x % kClusterCtas;
+  if (kCluster) {
+    u = blockIdx.x / kClusterCtas, u_end = u + 1;
+    if (u >= U) return;                                              // (the whole cluster: the grid is an upper bound)
+  } else {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    C = min(static_cast<int64_t>(gridDim.x), U);                    // every working CTA has at least one unit
+    const bool idle = blockIdx.x >= C;
+    u_end = idle ? 0 : share(blockIdx.x + 1, U, C);
+    u = idle ? 0 : share(blockIdx.x, U, C);
+  }
   bool first = true;
   Record rec = {};
   int b = 0;
@@ -382,10 +405,16 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     const int4 sq4 = seqs[b];
     const kv::Seq s{sq4.x, sq4.y, sq4.z, true};
     const int64_t nch = chunks_of(s), off = u - pre[b];
-    const uint32_t task = static_cast<uint32_t>(off < (1ll << 31) ? static_cast<uint32_t>(off) / static_cast<uint32_t>(nch)
-                                                                  : off / nch);
-    const int64_t ch0 = off - task * nch;
-    const int64_t ch1 = min(nch, ch0 + (u_end - u));
+    uint32_t task;
+    int64_t ch0, ch1;                                                // the run: chunks of 64 keys of the task
+    if (kCluster) {
+      task = static_cast<uint32_t>(off);
+      ch0 = nch * rank / kClusterCtas, ch1 = nch * (rank + 1) / kClusterCtas;
+    } else {
+      task = static_cast<uint32_t>(off < (1ll << 31) ? static_cast<uint32_t>(off) / static_cast<uint32_t>(nch) : off / nch);
+      ch0 = off - task * nch;
+      ch1 = min(nch, ch0 + (u_end - u));
+    }
     const uint32_t tile = task / a.hkv;
     const int h = static_cast<int>(task - tile * a.hkv.d);
     const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;    // rows of this K/V head
@@ -557,8 +586,9 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
                                                         acc.o[nt][2 * i + 1][k] * ou, acc.o[nt][2 * i + 1][k + 2] * ou);
       }
     __syncthreads();
-    const bool whole = ch0 == 0 && ch1 == nch;
-    float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * R * (HD + 2);
+    const bool whole = !kCluster && ch0 == 0 && ch1 == nch;
+    float* part = kCluster ? reinterpret_cast<float*>(smem + Cfg<NT>::kOut)
+                           : a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * R * (HD + 2);
     // a warp per row, 4 dims a lane
 #pragma unroll 2
     for (int row = warp; row < R; row += kWarps) {
@@ -582,6 +612,34 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
         reinterpret_cast<float4*>(part + row * HD)[lane] = o;
         if (lane == 0) part[R * HD + row] = m, part[R * HD + R + row] = l;
       }
+    }
+    if (kCluster) {
+      cluster_sync();
+      for (int i = warp; i < NT; i += kWarps) {                      // this CTA joins every eighth row
+        const int row = rank + kClusterCtas * i;
+        const uint32_t r = row0 + row, j = r / a.group;
+        if (r >= rows) break;
+        const uint32_t at = smem_u32(part);
+        float mj[kClusterCtas], lj[kClusterCtas], m = kNone, l = 0.0f;
+        float4 v[kClusterCtas], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kClusterCtas; ++k) {
+          const uint32_t remote = mapa_shared(at, k);
+          v[k] = ld_cluster4(remote + (row * HD + 4 * lane) * 4);
+          mj[k] = ld_cluster1(remote + (R * HD + row) * 4), lj[k] = ld_cluster1(remote + (R * HD + R + row) * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < kClusterCtas; ++k) m = fmaxf(m, mj[k]);
+#pragma unroll
+        for (int k = 0; k < kClusterCtas; ++k) {
+          const float f = exp2_approx(mj[k] - m);
+          l = fmaf(f, lj[k], l);
+          o.x = fmaf(f, v[k].x, o.x), o.y = fmaf(f, v[k].y, o.y), o.z = fmaf(f, v[k].z, o.z), o.w = fmaf(f, v[k].w, o.w);
+        }
+        store_row(a, s.s0 + j, h * a.group.d + r - j * a.group.d, lane, o, l);
+      }
+      cluster_sync();                                                // no CTA leaves while its piece is read
+      return;
     }
     if (!whole && ch0 == 0) {
       // the pieces end in the CTA that holds the task's last unit x: floor(j U / C) <= x < floor((j + 1) U / C)
@@ -681,16 +739,41 @@ inline int tile_n(int64_t T, int B, int group) {
 inline int ctas_of(int nt) { return sm_count() * (nt == 1 ? Cfg<1>::kCtas : nt == 2 ? Cfg<2>::kCtas : Cfg<4>::kCtas); }
 inline size_t part_bytes(int nt) { return static_cast<size_t>(ctas_of(nt)) * 2 * 8 * nt * (HD + 2) * 4; }
 
+// Clusters of the one-launch form: at most this many tasks, whatever the batch holds.
+inline int64_t tasks_of(int nt, int64_t T, int B, int group, int hkv) { return (T * group / (8 * nt) + B) * hkv; }
+
+template <int NT>
+inline int launch_cluster(const Args& a, int64_t tasks, cudaStream_t st) {
+  static PerDevice ready;
+  RL_TRY_CUDA(ready.once([] {
+    return cudaFuncSetAttribute(attend_kernel<NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch)));
+  }));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tasks * kClusterCtas));
+  cfg.blockDim = dim3(Cfg<NT>::kThreads);
+  cfg.dynamicSmemBytes = Cfg<NT>::smem(a.batch.B);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kClusterCtas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  RL_TRY_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<NT, true>, a));
+  return RL_OK;
+}
+
 template <int NT>
 inline int launch(const Args& a, cudaStream_t st) {
   const size_t smem = Cfg<NT>::smem(a.batch.B);
   const int ctas = ctas_of(NT);
   static PerDevice ready;
   RL_TRY_CUDA(ready.once([] {
-    return cudaFuncSetAttribute(attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(attend_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(Cfg<NT>::smem(kv::kMaxBatch)));
   }));
-  attend_kernel<NT><<<ctas, Cfg<NT>::kThreads, smem, st>>>(a);
+  attend_kernel<NT, false><<<ctas, Cfg<NT>::kThreads, smem, st>>>(a);
   RL_TRY_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);

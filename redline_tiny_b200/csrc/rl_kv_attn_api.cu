@@ -6,7 +6,7 @@
 namespace rl {
 namespace kvattn {
 
-inline int& path() {   // 0 = by the rule below, 1 = split kernel, 2 = prompt kernel
+inline int& path() {   // 0 = by the rules below, 1 = split kernel, 2 = prompt kernel, 3 = split kernel, in clusters
   static int v = 0;
   return v;
 }
@@ -15,13 +15,24 @@ inline int& path() {   // 0 = by the rule below, 1 = split kernel, 2 = prompt ke
 // the shape, gets through about a quarter of them: it pays where its tiles are more than a quarter full of rows and
 // the SMs more than a quarter full of tiles. (It scales row maxima, so it takes positive scales.)
 inline bool by_prompt(int64_t T, int B, int heads, int kv_heads, float scale_log2) {
-  if (!(scale_log2 > 0.0f) || path() == 1) return false;
+  if (!(scale_log2 > 0.0f) || path() == 1 || path() == 3) return false;
   if (path() == 2) return true;
   const int64_t rows = T * (heads / kv_heads), each = (rows + B - 1) / B;
   const int64_t tiles = (each + kvprompt::ROWS - 1) / kvprompt::ROWS * B;
   const double full = static_cast<double>(rows) / (static_cast<double>(tiles) * kvprompt::ROWS);
   const double busy = static_cast<double>(tiles * kv_heads) / sm_count();
   return full * (busy < 1.0 ? busy : 1.0) > 0.25;
+}
+
+// The one-launch form splits every task in eight, whatever its length: it wins while the page table bounds the keys and the
+// tasks' CTAs fit the GPU at once. Device times, spread over the grid / in clusters (32 heads over 8, one row a sequence):
+// 1 x 1024 keys 7.4 / 5.8 us, 1 x 4096 12.2 / 9.8, 1 x 8192 14.6 / 14.9, 2 x 8192 15.4 / 16.0, 8 x 4096 16.0 / 12.7,
+// 8 x 8192 20.7 / 19.0, 16 x 8192 34.5 / 35.4, 64 x 1024 33 / 53; 16 x up to 5 rows, 4097 keys, 8 over 2: 19.0 / 13.9.
+constexpr int64_t kShort = 6144;
+inline bool by_cluster(int nt, int64_t T, int B, int group, int hkv, int64_t most_keys) {
+  if (path() != 0) return path() == 3;
+  const int64_t tiles = (T * group + 8 * nt - 1) / (8 * nt);
+  return most_keys <= kShort && (tiles > B ? tiles : B) * hkv * kClusterCtas <= ctas_of(nt);
 }
 
 }  // namespace kvattn
@@ -88,6 +99,15 @@ int rl_kv_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, int64_t T, in
   const int nt = kvattn::tile_n(T, B, heads / kv_heads);
   a.part = static_cast<float*>(workspace);
   a.rec = reinterpret_cast<kvattn::Record*>(static_cast<uint8_t*>(workspace) + kvattn::part_bytes(nt));
+  const int group = heads / kv_heads;
+  if (kvattn::by_cluster(nt, T, B, group, kv_heads, table_ld * page)) {
+    const int64_t tasks = kvattn::tasks_of(nt, T, B, group, kv_heads);
+    switch (nt) {
+      case 1: return kvattn::launch_cluster<1>(a, tasks, stream);
+      case 2: return kvattn::launch_cluster<2>(a, tasks, stream);
+      default: return kvattn::launch_cluster<4>(a, tasks, stream);
+    }
+  }
   switch (nt) {
     case 1: return kvattn::launch<1>(a, stream);
     case 2: return kvattn::launch<2>(a, stream);

@@ -583,8 +583,8 @@ def set_attention_variant(v):
 
 
 def set_kv_attention_path(v):
-    """0 = by shape (default), 1 = the kernel that splits keys over the GPU, 2 = the tcgen05 prompt kernel; returns the
-    previous choice."""
+    """0 = by shape (default), 1 = the kernel that splits keys over the GPU, 2 = the tcgen05 prompt kernel, 3 = the
+    first in clusters, one launch; returns the previous choice."""
     return L.lib().rl_set_kv_attention_path(int(v))
 
 

@@ -21,11 +21,11 @@ def env():
     return torch, ops, _lib, torch.device("cuda:0")
 
 
-@pytest.fixture(params=["split", "prompt"])
+@pytest.fixture(params=["split", "prompt", "cluster"])
 def path(request, env):
-    """Both kernels of kv_attention take every shape."""
+    """Every kernel of kv_attention takes every shape."""
     ops = env[1]
-    before = ops.set_kv_attention_path({"split": 1, "prompt": 2}[request.param])
+    before = ops.set_kv_attention_path({"split": 1, "prompt": 2, "cluster": 3}[request.param])
     yield request.param
     ops.set_kv_attention_path(before)
 
@@ -446,14 +446,15 @@ def test_pages_behind_four_gigabytes(env, path):
 
 
 def test_the_kernel_goes_by_shape(env):
-    """A decode step takes the split kernel and a long chunk the prompt kernel; they agree within two weights' rounding and
-    the output's."""
+    """A decode step takes the split kernel, in clusters where the context is short, and a long chunk the prompt kernel; they
+    agree within two weights' rounding and the output's."""
     torch, ops, L, dev = env
-    for kv, new, H, hkv, which in (([500, 300], [1, 1], 8, 2, 1), ([900, 700], [900, 700], 32, 8, 2)):
+    for kv, new, H, hkv, which in (([500, 300], [1, 1], 8, 2, 3), ([6200, 300], [1, 1], 8, 2, 1),
+                                   ([900, 700], [900, 700], 32, 8, 2)):
         c = Case(torch, ops, dev, kv, new, hkv, 64, seed=41)
         q = bf16(torch, c.rng.standard_normal((c.T, H, 128)).astype(np.float32), dev)
         got = []
-        for path in (0, 1, 2):
+        for path in (0, 1, 2, 3):
             before = ops.set_kv_attention_path(path)
             got.append(ops.kv_attention(q, *c.args()))
             ops.set_kv_attention_path(before)
