@@ -429,15 +429,15 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint32_t rr = row0 + nt * 8 + 2 * c + k;
-        int64_t L = -1;
+        lim[nt][k] = INT32_MAX;                                      // rows behind the last: never stored, no reason to mask
         if (rr < rows) {
           const uint32_t j = rr / a.group;
-          L = s.len - s.n + j;
+          int64_t L = s.len - s.n + j;
           if (a.row_limit) L = min(s.len - 1, static_cast<int64_t>(__ldg(a.row_limit + s.s0 + j)));
+          lim[nt][k] = static_cast<int>(max(L, static_cast<int64_t>(-1)));
+          lim_max = max(lim_max, lim[nt][k]);
+          lim_min = min(lim_min, lim[nt][k]);
         }
-        lim[nt][k] = static_cast<int>(max(L, static_cast<int64_t>(-1)));
-        lim_max = max(lim_max, lim[nt][k]);
-        lim_min = min(lim_min, lim[nt][k]);
       }
     }
     lim_max = max(lim_max, __shfl_xor_sync(0xffffffffu, lim_max, 1));

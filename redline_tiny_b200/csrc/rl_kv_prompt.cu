@@ -13,7 +13,7 @@
 //    same layout read as MN-major B. The codes wait in the converters' registers for the time of a block (with one item in
 //    flight their latency bound the kernel: 791 us for the case below, staged through shared memory 346).
 //  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
-//  * the tile's rows need not be consecutive in memory, so Q is copied by the converter warps as well.
+//  * the tile's rows need not be consecutive in memory, so Q is copied by plain loads, all warps taking part.
 //
 // The softmax and its MMAs bound it: 4850 cycles per block of both tiles (3000 of them the softmax's, which shares the
 // issue slots and the shared memory with the converters; the dense kernel takes 3300 in all), the converters work 3300.
@@ -46,11 +46,11 @@ constexpr float kTau = 8.0f;
 constexpr int kConv = 3;              // converter warps: 0, 2 and 3 (1 issues the MMAs)
 
 struct Barriers {
-  uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_full, drain;
+  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_full, drain;
   uint32_t tmem_base;
   int abort;
   int e_max;                          // largest V exponent of the tile's keys
-  int task[4];                        // sequence, head, tile (or -1)
+  int task[6];                        // sequence (or -1), head, tile; the sequence's first row, rows and length
   int v_poison;                       // first position of the first V block with a NaN or an infinity
   alignas(8) uint8_t flag[RING][8];              // per block of 16 keys: 1 = K with a NaN or an infinity, 2 = absent
   alignas(16) float scale[RING][8];   // per block of 16 keys: what its raw scores are multiplied by
@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         const uint32_t t = static_cast<uint32_t>(at) / a.hkv;
         bars->task[1] = at - static_cast<int>(t) * a.pool.hkv;
         bars->task[2] = tiles - 1 - static_cast<int>(t);
+        bars->task[3] = static_cast<int>(s.s0), bars->task[4] = static_cast<int>(s.n), bars->task[5] = static_cast<int>(s.len);
       }
-      mbar_init(&bars->q_full, kConv);
       for (int i = 0; i < KS; ++i) mbar_init(&bars->k_full[i], kConv), mbar_init(&bars->k_empty[i], 1);
       for (int i = 0; i < VS; ++i) mbar_init(&bars->v_full[i], kConv), mbar_init(&bars->v_empty[i], 1);
       for (int t = 0; t < 2; ++t) {
@@ -286,56 +286,65 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   const uint32_t tmem = bars->tmem_base;
   const int h = bars->task[1];
   const uint32_t row0 = static_cast<uint32_t>(bars->task[2]) * ROWS;
-  const kv::Seq s = kv::load_seq(a.batch, b, a.pool.page);
+  const kv::Seq s{bars->task[3], bars->task[4], bars->task[5], true};
   const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;
   // the keys that any row sees: limits grow along the rows, unless row_limit gives them
   const uint32_t last_row = min(row0 + ROWS, rows) - 1;
   const int64_t kmax = a.row_limit ? s.len : s.len - s.n + last_row / a.group + 1;
   const int nblk = static_cast<int>((kmax + BKV - 1) / BKV);      // >= 1
 
+  // the page of the sequence's 16-key block u (-1 beyond the keys), and the block's pool index in it
+  const int32_t* table = a.batch.table + b * a.batch.ld;
+  const int units = static_cast<int>((kmax + BT - 1) / BT);
+  auto page_of = [&](int u) -> int { return u < units ? __ldg(table + (u >> (a.page_sh - 4))) : -1; };
+  auto present = [&](int pg) -> bool { return static_cast<uint32_t>(pg) < a.pool.pages; };
+  auto block_in = [&](int pg, int u) -> int {
+    return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + (u & ((1 << (a.page_sh - 4)) - 1));
+  };
+  {
+    // Q (256 rows x 16 chunks of 16 bytes) and the largest V exponent, by all warps and with the loads ahead of the stores:
+    // this start is paid per task (the converters alone, a load at a time, took 15 us to the first product)
+    constexpr int kQLoads = (ROWS * 16 + kThreads - 1) / kThreads;
+    uint4 v[kQLoads];
+#pragma unroll
+    for (int i = 0; i < kQLoads; ++i) {
+      const int x = threadIdx.x + i * kThreads;
+      const uint32_t rr = row0 + (x >> 4);
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (x < ROWS * 16 && rr < rows) {
+        const uint32_t j = rr / a.group;
+        v[i] = *reinterpret_cast<const uint4*>(a.q + (s.s0 + j) * a.q_st + (h * a.group.d + rr - j * a.group.d) * a.q_sh +
+                                               8 * (x & 15));
+      }
+    }
+    int e = 0;
+#pragma unroll 2
+    for (int u = threadIdx.x; u < units; u += kThreads) {
+      const int pg = page_of(u);
+      if (!present(pg)) {
+        report(kErrBadArgument);
+        continue;
+      }
+      const int ve = a.pool.ve[block_in(pg, u)];
+      if (ve != 255) e = max(e, ve);
+      else atomicMin(&bars->v_poison, u * BT);
+    }
+    e = __reduce_max_sync(0xffffffffu, e);
+    if (lane == 0) atomicMax(&bars->e_max, e);
+#pragma unroll
+    for (int i = 0; i < kQLoads; ++i) {
+      const int x = threadIdx.x + i * kThreads, r = x >> 4, c = x & 15, y = r & 127;
+      if (x < ROWS * 16)
+        *reinterpret_cast<uint4*>(smem + kQ + (r >> 7) * TILE + (c >> 3) * SUB + y * 128 + (((c & 7) ^ (y & 7)) << 4)) = v[i];
+    }
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+
   if (warp < 4) {
     if (warp != 1) {
       // ---------------- converters ----------------
       const int cw = warp == 0 ? 0 : warp - 1;
-      // the page of the sequence's 16-key block u (-1 beyond the keys), and the block's pool index in it
-      const int32_t* table = a.batch.table + b * a.batch.ld;
-      const int units = static_cast<int>((kmax + BT - 1) / BT);
-      auto page_of = [&](int u) -> int { return u < units ? __ldg(table + (u >> (a.page_sh - 4))) : -1; };
-      auto present = [&](int pg) -> bool { return static_cast<uint32_t>(pg) < a.pool.pages; };
-      auto block_in = [&](int pg, int u) -> int {
-        return ((pg * a.pool.hkv + h) << (a.page_sh - 4)) + (u & ((1 << (a.page_sh - 4)) - 1));
-      };
-      // the largest V exponent
-      int e = 0;
-#pragma unroll 4
-      for (int u = cw * 32 + lane; u < units; u += kConv * 32) {
-        const int pg = page_of(u);
-        if (!present(pg)) {
-          report(kErrBadArgument);
-          continue;
-        }
-        const int ve = a.pool.ve[block_in(pg, u)];
-        if (ve != 255) e = max(e, ve);
-        else atomicMin(&bars->v_poison, u * BT);
-      }
-      e = __reduce_max_sync(0xffffffffu, e);
-      if (lane == 0) atomicMax(&bars->e_max, e);
-      // Q: 256 rows x 16 chunks of 16 bytes
-      for (int i = cw * 32 + lane; i < ROWS * 16; i += kConv * 32) {
-        const int r = i >> 4, c = i & 15;
-        const uint32_t rr = row0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (rr < rows) {
-          const uint32_t j = rr / a.group;
-          v = *reinterpret_cast<const uint4*>(a.q + (s.s0 + j) * a.q_st + (h * a.group.d + rr - j * a.group.d) * a.q_sh + 8 * c);
-        }
-        const int x = r & 127;
-        *reinterpret_cast<uint4*>(smem + kQ + (r >> 7) * TILE + (c >> 3) * SUB + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->q_full);
-      asm volatile("bar.sync 1, 96;" ::: "memory");               // the converters' maxima are joined
       const int em = bars->e_max;
 
       // Warp cw converts units cw, cw + 3 and cw + 6 of each block's eight. The codes of block j + 1 are loaded into
@@ -441,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         }
         return true;
       };
-      bool ok = mbar_wait_warp(&bars->q_full, 0, abort) && qk(0, 0) && qk(1, 0);
+      bool ok = qk(0, 0) && qk(1, 0);
       for (int j = 1; ok && j < nblk; ++j) ok = pv(0, j - 1) && qk(0, j) && pv(1, j - 1) && qk(1, j);
       if (ok) ok = pv(0, nblk - 1) && pv(1, nblk - 1);
       if (elect_one()) {
@@ -460,11 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     const uint32_t lane_off = (32u * q) << 16;
     const uint32_t ta = tmem + t * BKV + lane_off, to = tmem + kOCol + t * HD + lane_off;
     const uint32_t jr = row / a.group;
-    int lim = -1;
-    if (row < rows) {
-      lim = static_cast<int>(s.len - s.n + jr);
-      if (a.row_limit) lim = min(static_cast<int>(s.len) - 1, __ldg(a.row_limit + s.s0 + jr));
-    }
+    // (rows behind the last, which are not stored, see what it sees: a mask in every block would cost their warp 1000 cycles)
+    const uint32_t jl = min(jr, static_cast<uint32_t>(s.n) - 1);
+    int lim = static_cast<int>(s.len - s.n + jl);
+    if (a.row_limit) lim = min(static_cast<int>(s.len) - 1, __ldg(a.row_limit + s.s0 + jl));
     float m_run = -INFINITY, l_run = 0.0f;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
