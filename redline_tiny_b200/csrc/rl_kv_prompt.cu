@@ -412,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       constexpr uint32_t idesc_o = idesc_f16_bmn(BQ, HD);
       bool any = false;
       const uint32_t qa0 = smem_u32(smem + kQ);
-      auto qk = [&](int t, int j) -> bool {
+      auto k_ready = [&](int j) -> bool { return mbar_wait_warp(&bars->k_full[j % KS], (j / KS) & 1, abort); };
+      auto qk = [&](int t, int j) {
         const int st = j % KS;
-        if (!mbar_wait_warp(&bars->k_full[st], (j / KS) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t qa = qa0 + t * TILE, kb = smem_u32(smem + kK + st * TILE);
         if (elect_one()) {
@@ -429,7 +429,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         }
         __syncwarp();
         any = true;
-        return true;
       };
       auto pv = [&](int t, int j) -> bool {
         const int st = j % VS;
@@ -437,6 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         const uint32_t vb = smem_u32(smem + kV + st * TILE);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
+          // (K of the product behind this one is waited for here, where the wait is hidden)
+          if (hh == 1 && j + 1 < nblk && !k_ready(j + 1)) return false;
           if (!mbar_wait_warp(&bars->p_full[t][hh], j & 1, abort)) return false;
           tc_fence_after();
           if (elect_one()) {
@@ -450,9 +451,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         }
         return true;
       };
-      bool ok = qk(0, 0) && qk(1, 0);
-      for (int j = 1; ok && j < nblk; ++j) ok = pv(0, j - 1) && qk(0, j) && pv(1, j - 1) && qk(1, j);
-      if (ok) ok = pv(0, nblk - 1) && pv(1, nblk - 1);
+      bool ok = k_ready(0);
+      if (ok) qk(0, 0), qk(1, 0);
+      for (int j = 0; ok && j < nblk; ++j)
+        for (int t = 0; ok && t < 2; ++t) {
+          ok = pv(t, j);
+          if (ok && j + 1 < nblk) qk(t, j + 1);
+        }
       if (elect_one()) {
         if (ok) umma_commit(&bars->o_full);
         if (!ok && any) {
