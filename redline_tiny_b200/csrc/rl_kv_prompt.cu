@@ -15,11 +15,16 @@
 //  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
 //  * the tile's rows need not be consecutive in memory, so Q is copied by plain loads, all warps taking part.
 //
-// The softmax and its MMAs bound it: 4850 cycles per block of both tiles (3000 of them the softmax's, which shares the
-// issue slots and the shared memory with the converters; the dense kernel takes 3300 in all), the converters work 3300.
-// Three prompt chunks of 1021, 650 and 279 tokens over 8191, 5214 and 2245 (32 heads over 8): 267 us, 713 TFLOP/s; a fifth
-// of it is the tail of 256 tiles of three lengths on 148 SMs. Rejected: reading S twice to free registers (361 - 424 us),
-// the scales read from shared memory where they are used (280 us).
+// The chain of a tile bounds it, 4000 cycles per block of both tiles: softmax 2700 (it shares the issue slots and the shared
+// memory with the converters), the rest of P V and the next S 1300, about twice their arithmetic, since their operands and
+// the converters' stores share the shared memory too (the dense kernel takes 3300). A task adds 5.5 us until its first S and
+// about 2 behind its last block.
+// Three prompt chunks of 1021, 650 and 279 tokens over 8191, 5214 and 2245 (32 heads over 8): 233 us, 816 TFLOP/s; a fifth
+// of it is the tail of 256 tasks of three lengths on 148 SMs. Steps: Q and the exponents by the converters alone, 272; by
+// all warps, loads ahead of stores, 242; the wait for K taken off the chain, 233. Rejected: reading S twice to free
+// registers (361 - 424 against 267), scales read from shared memory where they are used (280), part of the exponentials by a
+// polynomial (289 - 311 against 279), four converter warps (487), P handed over as 96 + 32 keys (248 against 233) or in
+// quarters (236), one thread for the issuer's waits (240), the first codes loaded ahead of the start's barrier (266).
 #include "rl_common.cuh"
 #include "rl_host.h"
 
