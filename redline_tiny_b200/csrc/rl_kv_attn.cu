@@ -6,7 +6,7 @@
 // 2^-28 of it) times one fp32 factor per block and row. P is rounded to fp16 (11 significant bits, half a step 2^-11
 // of each weight; the row sum adds them unrounded). P . mv, again with exact integers, accumulates in fp32 in units of
 // 2^(er-133), er the largest V exponent so far; a block's own scale 2^(ev-er) goes into its P. So the only roundings are
-// P's and fp32's.
+// P's and fp32's. A row keeps the er of the last block that it sees, so that no hidden key reaches it.
 //
 // The rows of one K/V head that share its keys (tokens of a sequence x query heads of the group) are the N side of
 // mma.m16n8k16: S^T (16 tokens x 8 rows) = K q~^T and O^T (16 dims x 8 rows) += V^T P^T. The cache is then the A
@@ -172,7 +172,14 @@ template <int NT>
 struct Acc {
   float o[NT][8][4];     // O^T: dims 16g + 2i (+1 for [2], [3]), rows 2c, 2c + 1 of n-tile nt
   float m[NT][2], l[NT][2];
-  int er;                // O is in units of 2^(er - 133)
+  int er;                // the largest V exponent of the warp's blocks so far
+  uint32_t unit[(NT + 1) / 2];   // O of a row is in units of 2^(unit - 133), a byte a row: er of the last block that it sees
+
+  __device__ __forceinline__ int unit_of(int nt, int c) const { return unit[nt >> 1] >> (16 * (nt & 1) + 8 * c) & 255u; }
+  __device__ __forceinline__ void set_unit(int nt, int c, int e) {
+    const int sh = 16 * (nt & 1) + 8 * c;
+    unit[nt >> 1] = (unit[nt >> 1] & ~(255u << sh)) | static_cast<uint32_t>(e) << sh;
+  }
 };
 
 // P^T of a block times 2^shift, in the B layout; the row sums add the weights, before their rounding, times `unit`.
@@ -252,10 +259,16 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
     change |= fmaxf(s[nt][0], s[nt][2]) > acc.m[nt][0] + kRaise || fmaxf(s[nt][1], s[nt][3]) > acc.m[nt][1] + kRaise;
   }
   if (__any_sync(0xffffffffu, change)) {
+    // (a row that does not see this block, nor any behind it, keeps its unit: what is hidden may be 2^200 times its values)
     float to = 1.0f;
     if (ev > acc.er) {
       to = exp2f(static_cast<float>(acc.er - ev));
       acc.er = ev;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (pos0 <= lim[nt][c]) acc.set_unit(nt, c, ev);
     }
     d = acc.er - ev;
 #pragma unroll
@@ -270,7 +283,7 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
         const float alpha = m == acc.m[nt][c] ? 1.0f : exp2_approx(acc.m[nt][c] - m);
         acc.m[nt][c] = m;
         acc.l[nt][c] *= alpha;
-        const float f = alpha * to;
+        const float f = pos0 <= lim[nt][c] ? alpha * to : alpha;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           acc.o[nt][i][c] *= f;
@@ -540,6 +553,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     Acc<NT> acc;
     acc.er = 0;
 #pragma unroll
+    for (int i = 0; i < (NT + 1) / 2; ++i) acc.unit[i] = 0;
+#pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       acc.m[nt][0] = acc.m[nt][1] = kNone;
       acc.l[nt][0] = acc.l[nt][1] = 0.0f;
@@ -567,7 +582,6 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     cp_wait<0>();
     __syncthreads();           // every warp is done with the ring
 
-    const float ou = bfp16_scale(static_cast<uint32_t>(acc.er));
     // join the warps: (O, m, l) of each through shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -578,6 +592,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = nt * 8 + 2 * c + k;
+        const float ou = bfp16_scale(static_cast<uint32_t>(acc.unit_of(nt, k)));
         if (g == 0) sm[warp * R + row] = acc.m[nt][k], sl[warp * R + row] = l;
         float* d = so + (warp * R + row) * HD + 16 * g;
 #pragma unroll

@@ -1,0 +1,74 @@
+"""GPU parity of the attention over the 8-bit paged cache (rl_kv_attention) at the ends of its numeric range: values whose
+scales lie far apart, values near the largest float, long tails of small weights.
+
+|o - ref| <= the bound of oracle/cache_oracle.py, which is relative to the largest value that the ROW sees, plus half a bf16
+step, 2^-8 |ref|, of the output's rounding. A key that the mask hides from a row must not reach the row in any form."""
+
+import numpy as np
+import pytest
+
+from oracle import bfp16_oracle as O
+from test_gpu_kv_cache import Case, bf16, check_attention
+
+pytestmark = pytest.mark.gpu
+
+FORMS = {"split": 1, "prompt": 2, "cluster": 3}
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+    from redline_tiny_b200 import _lib, ops
+    assert torch.cuda.is_available()
+    return torch, ops, _lib, torch.device("cuda:0")
+
+
+def attend(ops, form, *args, **kw):
+    before = ops.set_kv_attention_path(FORMS[form])
+    try:
+        return ops.kv_attention(*args, **kw)
+    finally:
+        ops.set_kv_attention_path(before)
+
+
+def value_exponents(c, torch, dev, exps):
+    """Give the blocks of sequence b's values the exponents exps(b, first position of the block)."""
+    for b in range(len(c.kv)):
+        for pos in range(0, c.kv[b], 16):
+            c.v.exps[c.table[b, pos // c.page], :, pos % c.page // 16] = exps(b, pos)
+    c.pool.v_exp[c.layer] = torch.from_numpy(c.v.exps).to(dev)
+
+
+def limits(c, rng, at):
+    """Row limits: nothing, one key, and keys up to and beyond position `at`."""
+    lim = rng.integers(-1, max(c.kv), c.T)
+    lim[::3] = rng.integers(0, at, len(lim[::3]))
+    lim[1::7] = -1
+    return lim.astype(np.int32)
+
+
+def hidden_values(env, form, spread, masks, kv, new, H, hkv, page):
+    """From position 192 on, values 2^spread times the others: the rows that see none of them keep their own scale."""
+    torch, ops, L, dev = env
+    c = Case(torch, ops, dev, kv, new, hkv, page, seed=spread + H)
+    low = 120 - spread // 2
+    value_exponents(c, torch, dev, lambda b, pos: low + spread if pos >= 192 else low)
+    q = O.bf16_round(c.rng.standard_normal((c.T, H, 128)).astype(np.float32))
+    lim = limits(c, c.rng, 192) if masks == "row_limit" else None
+    got = attend(ops, form, bf16(torch, q, dev), *c.args(), row_limit=None if lim is None else torch.from_numpy(lim).to(dev))
+    ops.device_status()
+    ref, tol = c.oracle(q, lim)
+    sees = np.concatenate([a - n + np.arange(n) for a, n in zip(kv, new)]) if lim is None else lim
+    below = ref[(sees >= 0) & (sees < 192)]
+    assert len(below) and np.abs(below).max() > 0
+    check_attention(got, ref, tol)
+
+
+HIDDEN = [([300], [300], 2, 1, 16), ([700, 250], [600, 130], 4, 2, 64)]
+
+
+@pytest.mark.parametrize("kv,new,H,hkv,page", HIDDEN)
+@pytest.mark.parametrize("masks", ["causal", "row_limit"])
+@pytest.mark.parametrize("form", ["split", "cluster"])
+def test_hidden_values_far_above(env, form, masks, kv, new, H, hkv, page):
+    hidden_values(env, form, 180, masks, kv, new, H, hkv, page)
