@@ -40,6 +40,9 @@ constexpr float kRaise = 8.0f;   // the running maximum rises only when a score 
 constexpr int kUp = 4;
 constexpr uint32_t kWindow = 8;
 constexpr float kNone = -1e30f;  // running maximum before any key (finite: no inf - inf)
+// Pieces are joined in float, weights up to 2^12 and their sums included. A row whose unit is above 2^(kMostUnit - 133) is
+// joined 2^x smaller, its sum too and its maximum x larger, which is the same piece: x = unit - kMostUnit.
+constexpr int kMostUnit = 190;
 
 // n / d for 0 <= n < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d), s = ceil(log2 d); mul d exceeds
 // 2^(31 + s) by e < d <= 2^s, so n e < 2^(31 + s) and the quotient is exact.
@@ -592,8 +595,10 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = nt * 8 + 2 * c + k;
-        const float ou = bfp16_scale(static_cast<uint32_t>(acc.unit_of(nt, k)));
-        if (g == 0) sm[warp * R + row] = acc.m[nt][k], sl[warp * R + row] = l;
+        const int unit = acc.unit_of(nt, k), over = max(unit - kMostUnit, 0);
+        const float ou = bfp16_scale(static_cast<uint32_t>(unit - over));
+        l *= __uint_as_float(static_cast<uint32_t>(127 - over) << 23);
+        if (g == 0) sm[warp * R + row] = acc.m[nt][k] + static_cast<float>(over), sl[warp * R + row] = l;
         float* d = so + (warp * R + row) * HD + 16 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i)

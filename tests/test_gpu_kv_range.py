@@ -72,3 +72,16 @@ HIDDEN = [([300], [300], 2, 1, 16), ([700, 250], [600, 130], 4, 2, 64)]
 @pytest.mark.parametrize("form", ["split", "cluster"])
 def test_hidden_values_far_above(env, form, masks, kv, new, H, hkv, page):
     hidden_values(env, form, 180, masks, kv, new, H, hkv, page)
+
+
+@pytest.mark.parametrize("kv,new,H", [([3000], [1], 4), ([2000, 900], [40, 300], 2)])
+@pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
+def test_values_near_the_largest(env, form, kv, new, H):
+    """Values up to 2^127 over thousands of keys: the sum of weights does not overflow the sum of values."""
+    torch, ops, L, dev = env
+    c = Case(torch, ops, dev, kv, new, 1, 64, seed=3)
+    value_exponents(c, torch, dev, lambda b, pos: 254 - pos // 16 % 3)
+    q = O.bf16_round((c.rng.standard_normal((c.T, H, 128)) * 0.1).astype(np.float32))
+    got = attend(ops, form, bf16(torch, q, dev), *c.args())
+    ops.device_status()
+    check_attention(got, *c.oracle(q))
