@@ -129,6 +129,29 @@ __device__ __forceinline__ void cp_wait() {
 // (a plain load, which the compiler may place among the matrix instructions)
 __device__ __forceinline__ uint4 lds128(const uint8_t* a) { return *reinterpret_cast<const uint4*>(a); }
 
+// A row's q (the lane's dims 16c.. and 64 + 16c..) as fp16 times 2^(141 - e), which puts the row's largest value in
+// [2^14, 2^15). Returns e, its exponent field.
+__device__ __forceinline__ uint32_t q_fragments(const uint4 (&w)[4], uint32_t (&qf)[16]) {
+  const uint32_t x[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
+                          w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx = max(mx, max(x[i] & 0x7FFFu, x[i] >> 16 & 0x7FFFu));
+  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  const uint32_t e = max(mx >> 7, 32u);                              // (values below 2^-95 keep less)
+  const float up = __uint_as_float((268u - e) << 23);
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    qf[i] = pack_h2(__uint_as_float(x[i] << 16) * up, __uint_as_float(x[i] & 0xFFFF0000u) * up);
+  return e;
+}
+// What the scores of row k (of the lanes that hold e) are multiplied by: 2^(e - 141) scale.
+__device__ __forceinline__ float q_scale(uint32_t e, int row, float scale_log2) {
+  const int er = __shfl_sync(0xffffffffu, static_cast<int>(e), row * 4);
+  return __uint_as_float(static_cast<uint32_t>(er - 14) << 23) * scale_log2;
+}
+
 // The list of units: sequence b has hkv * tiles(b) tasks of chunks(b) units each.
 __device__ __forceinline__ int64_t tiles_of(const Args& a, const kv::Seq& s, int R) {
   return (s.n * a.group.d + R - 1) / R;
@@ -524,19 +547,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     // q of the tile, while the first blocks are on their way
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint4 (&w)[4] = qw[nt];
-      const uint32_t x[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
-                              w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
-      uint32_t mx = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = max(mx, max(x[i] & 0x7FFFu, x[i] >> 16 & 0x7FFFu));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const uint32_t e = max(mx >> 7, 32u);                          // exponent field (values below 2^-95 keep less)
-      const float up = __uint_as_float((268u - e) << 23);            // 2^(141 - e)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        qf[i] = pack_h2(__uint_as_float(x[i] << 16) * up, __uint_as_float(x[i] & 0xFFFF0000u) * up);
+      const uint32_t e = q_fragments(qw[nt], qf);
       if (NT > 1 && nt % kWarps == warp) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -544,10 +555,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
               make_uint4(qf[4 * i], qf[4 * i + 1], qf[4 * i + 2], qf[4 * i + 3]);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int ec = __shfl_sync(0xffffffffu, static_cast<int>(e), (2 * c + k) * 4);
-        qs[nt][k] = __uint_as_float(static_cast<uint32_t>(ec - 14) << 23) * a.scale_log2;   // 2^(e - 141)
-      }
+      for (int k = 0; k < 2; ++k) qs[nt][k] = q_scale(e, 2 * c + k, a.scale_log2);
     }
 
     if (NT > 1) __syncthreads();

@@ -7,9 +7,12 @@
 //
 //  * three converter warps read the pages' codes and write the MMA operands into shared memory. K: bf16 (u - 128) / 64,
 //    exact (a byte taken as bf16 bits is u 2^-133, so one FMA scales it and takes the offset off); the block's scale
-//    2^(ek - 133) is applied to S, 16 columns at a time, where the softmax scales them anyway. V: fp16 (u - 128) 2^(ev - e),
-//    exact down to 2^-24, with e the largest V exponent that the tile sees, found before the first block; O is multiplied by
-//    2^(e - 133) at the end. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
+//    2^(ek - 133) is applied to S, 16 columns at a time, where the softmax scales them anyway. V: fp16 (u - 128) 2^(5 + ev - e),
+//    exact down to 2^-24, with e the largest V exponent that any row of the tile sees, found before the first block; O is
+//    multiplied by 2^(e - 138) at the end. Blocks more than kReach = 29 below e become zeros (they hold less than 2^-29 of
+//    the largest value that e admits). That is done only while every row sees a block of e or e - 1; elsewhere a tile with
+//    blocks that far down goes by the split kernel's steps (far_tile), whose unit is each row's own, so that no hidden key
+//    reaches a row. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
 //    same layout read as MN-major B. The codes wait in the converters' registers for the time of a block (with one item in
 //    flight their latency bound the kernel: 791 us for the case below, staged through shared memory 346).
 //  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
@@ -48,13 +51,17 @@ constexpr int kBytes = 1024 + kBar + 1024;
 static_assert(kBytes <= 232448, "shared memory");
 constexpr int kTmemCols = 512, kOCol = 256;
 constexpr float kTau = 8.0f;
+constexpr int kUpV = 5;               // V is kept times 2^kUpV: 1152 2^kUpV, the offset, has to be an fp16 number
+constexpr int kReach = 24 + kUpV;
 constexpr int kConv = 3;              // converter warps: 0, 2 and 3 (1 issues the MMAs)
 
 struct Barriers {
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2][2], o_full, drain;
   uint32_t tmem_base;
   int abort;
-  int e_max;                          // largest V exponent of the tile's keys
+  int e_max, e_min;                   // largest and smallest V exponent of the tile's keys
+  int e_all;                          // largest V exponent of the blocks that every row (with any key) sees
+  int lim_min, lim_max;               // the smallest and largest limit of its rows (with any key)
   int task[6];                        // sequence (or -1), head, tile; the sequence's first row, rows and length
   int v_poison;                       // first position of the first V block with a NaN or an infinity
   alignas(8) uint8_t flag[RING][8];              // per block of 16 keys: 1 = K with a NaN or an infinity, 2 = absent
@@ -219,7 +226,83 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
   l_run += a.x + a.y;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
+// The last key that new token j of a sequence sees (-1: none).
+__device__ __forceinline__ int limit_of(const Args& a, const kv::Seq& s, uint32_t j) {
+  if (!a.row_limit) return static_cast<int>(s.len - s.n + j);
+  return max(-1, min(static_cast<int>(s.len) - 1, __ldg(a.row_limit + s.s0 + j)));
+}
+
+// A tile whose values lie too far apart for one fp16 unit (rare): eight rows a warp, over all their keys, block by block as
+// the split kernel does. Right for every tile, at a small part of the rate.
+__device__ __noinline__ void far_tile(const Args& a, const int (&task)[6]) {
+  const int b = task[0], h = task[1];
+  const kv::Seq s{task[3], task[4], task[5], true};
+  const uint32_t row0 = static_cast<uint32_t>(task[2]) * ROWS, rows = static_cast<uint32_t>(s.n) * a.group.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int32_t* table = a.batch.table + b * a.batch.ld;
+  const uint32_t end = min(rows, row0 + ROWS);
+  for (uint32_t r0 = row0 + 8 * warp; r0 < end; r0 += 8 * (kThreads / 32)) {
+    uint4 qw[4] = {};
+    if (r0 + g < end) {
+      const uint32_t j = (r0 + g) / a.group;
+      const uint16_t* p = a.q + (s.s0 + j) * a.q_st + (h * a.group.d + r0 + g - j * a.group.d) * a.q_sh + 16 * c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qw[i] = *reinterpret_cast<const uint4*>(p + 64 * (i >> 1) + 8 * (i & 1));
+    }
+    uint32_t qf[16];
+    const uint32_t e = kvattn::q_fragments(qw, qf);
+    float qs[1][2];
+    int lim[1][2], lim_min = INT32_MAX, lim_max = -1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t r = r0 + 2 * c + k;
+      qs[0][k] = kvattn::q_scale(e, 2 * c + k, a.scale_log2);
+      lim[0][k] = INT32_MAX;                                         // (rows behind the last are not stored)
+      if (r < end) {
+        lim[0][k] = limit_of(a, s, r / a.group);
+        lim_min = min(lim_min, lim[0][k]), lim_max = max(lim_max, lim[0][k]);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+      lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
+      lim_max = max(lim_max, __shfl_xor_sync(0xffffffffu, lim_max, d));
+    }
+    kvattn::Acc<1> acc = {};
+    acc.m[0][0] = acc.m[0][1] = kvattn::kNone;
+    for (int u = 0; u * BT <= lim_max; ++u) {
+      const int pg = __ldg(table + (u >> (a.page_sh - 4)));
+      if (static_cast<uint32_t>(pg) >= a.pool.pages) continue;       // (reported at the tile's start)
+      const int64_t blk = (static_cast<int64_t>(pg * a.pool.hkv + h) << (a.page_sh - 4)) + (u & ((1 << (a.page_sh - 4)) - 1));
+      const uint8_t* kp = a.pool.k + blk * (BT * HD) + g * HD + 16 * c;
+      const uint8_t* vp = a.pool.v + blk * (BT * HD) + 2 * c * HD + 16 * g;
+      uint4 kr[4], vr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kr[i] = *reinterpret_cast<const uint4*>(kp + (i >> 1) * 8 * HD + (i & 1) * 64);
+        vr[i] = *reinterpret_cast<const uint4*>(vp + (i >> 1) * 8 * HD + (i & 1) * HD);
+      }
+      kvattn::block_step<1>(kr, vr, a.pool.ke[blk], a.pool.ve[blk], u * BT, qf, nullptr, qs, lim, lim_min, g, acc);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float l = acc.l[0][k];
+#pragma unroll
+      for (int d = 4; d <= 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      const uint32_t r = r0 + 2 * c + k, j = r / a.group;
+      if (r >= end) continue;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = bfp16_scale(static_cast<uint32_t>(acc.unit_of(0, k)));
+      uint16_t* o = a.o + (s.s0 + j) * a.ldo + (h * a.group.d + r - j * a.group.d) * HD + 16 * g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          o[2 * i + y] = __bfloat16_as_ushort(__float2bfloat16_rn(acc.o[0][i][k + 2 * y] * inv * unit));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Barriers* bars = reinterpret_cast<Barriers*>(smem + kBar);
@@ -273,7 +356,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       mbar_init(&bars->o_full, 1);
       mbar_init(&bars->drain, 1);
       bars->abort = 0;
-      bars->e_max = 0;
+      bars->e_max = bars->e_all = 0;
+      bars->e_min = 255;
+      bars->lim_min = INT32_MAX, bars->lim_max = -1;
       bars->v_poison = INT32_MAX;
       fence_mbar_init();
     }
@@ -281,6 +366,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   __syncthreads();
   const int b = bars->task[0];
   if (b < 0) return;   // (the grid is an upper bound)
+  const int h = bars->task[1];
+  const uint32_t row0 = static_cast<uint32_t>(bars->task[2]) * ROWS;
+  const kv::Seq s{bars->task[3], bars->task[4], bars->task[5], true};
+  const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;
+  const uint32_t last_row = min(row0 + ROWS, rows) - 1;
+  if (a.row_limit && warp < ROWS / 32) {
+    const uint32_t r = row0 + threadIdx.x;
+    const int L = r <= last_row ? limit_of(a, s, r / a.group) : -1;
+    const int lo = __reduce_min_sync(0xffffffffu, L < 0 ? INT32_MAX : L), hi = __reduce_max_sync(0xffffffffu, L);
+    if (lane == 0) atomicMin(&bars->lim_min, lo), atomicMax(&bars->lim_max, hi);
+  }
   if (warp == 0) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
@@ -289,18 +385,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  const int h = bars->task[1];
-  const uint32_t row0 = static_cast<uint32_t>(bars->task[2]) * ROWS;
-  const kv::Seq s{bars->task[3], bars->task[4], bars->task[5], true};
-  const uint32_t rows = static_cast<uint32_t>(s.n) * a.group.d;
-  // the keys that any row sees: limits grow along the rows, unless row_limit gives them
-  const uint32_t last_row = min(row0 + ROWS, rows) - 1;
-  const int64_t kmax = a.row_limit ? s.len : s.len - s.n + last_row / a.group + 1;
-  const int nblk = static_cast<int>((kmax + BKV - 1) / BKV);      // >= 1
+  // the keys that any row sees, and those that every row sees which sees any: limits grow along the rows, unless row_limit
+  // gives them
+  const int kmax = a.row_limit ? max(bars->lim_max, 0) + 1 : limit_of(a, s, last_row / a.group) + 1;
+  const int lim_all = a.row_limit ? bars->lim_min : limit_of(a, s, row0 / a.group);
+  const int nblk = (kmax + BKV - 1) / BKV;                        // >= 1
 
   // the page of the sequence's 16-key block u (-1 beyond the keys), and the block's pool index in it
   const int32_t* table = a.batch.table + b * a.batch.ld;
-  const int units = static_cast<int>((kmax + BT - 1) / BT);
+  const int units = (kmax + BT - 1) / BT;
   auto page_of = [&](int u) -> int { return u < units ? __ldg(table + (u >> (a.page_sh - 4))) : -1; };
   auto present = [&](int pg) -> bool { return static_cast<uint32_t>(pg) < a.pool.pages; };
   auto block_in = [&](int pg, int u) -> int {
@@ -322,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
                                                8 * (x & 15));
       }
     }
-    int e = 0;
+    int e = 0, e_all = 0, e_min = 255;
 #pragma unroll 2
     for (int u = threadIdx.x; u < units; u += kThreads) {
       const int pg = page_of(u);
@@ -331,11 +424,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         continue;
       }
       const int ve = a.pool.ve[block_in(pg, u)];
-      if (ve != 255) e = max(e, ve);
-      else atomicMin(&bars->v_poison, u * BT);
+      if (ve != 255) {
+        e = max(e, ve), e_min = min(e_min, ve);
+        if (u * BT <= lim_all) e_all = max(e_all, ve);
+      } else {
+        atomicMin(&bars->v_poison, u * BT);
+      }
     }
     e = __reduce_max_sync(0xffffffffu, e);
-    if (lane == 0) atomicMax(&bars->e_max, e);
+    e_all = __reduce_max_sync(0xffffffffu, e_all);
+    e_min = __reduce_min_sync(0xffffffffu, e_min);
+    if (lane == 0) atomicMax(&bars->e_max, e), atomicMax(&bars->e_all, e_all), atomicMin(&bars->e_min, e_min);
 #pragma unroll
     for (int i = 0; i < kQLoads; ++i) {
       const int x = threadIdx.x + i * kThreads, r = x >> 4, c = x & 15, y = r & 127;
@@ -346,7 +445,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   }
   __syncthreads();
 
-  if (warp < 4) {
+  if (bars->e_max - bars->e_min > kReach && bars->e_max - bars->e_all > 1) {
+    far_tile(a, bars->task);
+  } else if (warp < 4) {
     if (warp != 1) {
       // ---------------- converters ----------------
       const int cw = warp == 0 ? 0 : warp - 1;
@@ -397,10 +498,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         if (!mbar_wait_warp(&bars->v_empty[vs], ((j / VS) & 1) ^ 1, abort)) break;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          // 2^-d and -1152 2^-d in fp16. P = 0 for keys beyond the end or absent; a poisoned block's codes count as
+          // 2^(kUpV - d) and -1152 times it in fp16. P = 0 for keys beyond the end or absent; a poisoned block's codes count as
           // they are (the rows that see it become NaN).
           const int d = vu[i].e == 255u ? 0 : em - static_cast<int>(vu[i].e & 255u);
-          const float f = d > 24 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - d) << 23);
+          const float f = d > kReach ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + kUpV - d) << 23);
           if (cw + 3 * i < 8)
             write_unit<true>(smem + kV + vs * TILE, 16 * (cw + 3 * i), vu[i], kvattn::pack_h2(f, f),
                              kvattn::pack_h2(-1152.0f * f, -1152.0f * f), lane);
@@ -481,8 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     const uint32_t jr = row / a.group;
     // (rows behind the last, which are not stored, see what it sees: a mask in every block would cost their warp 1000 cycles)
     const uint32_t jl = min(jr, static_cast<uint32_t>(s.n) - 1);
-    int lim = static_cast<int>(s.len - s.n + jl);
-    if (a.row_limit) lim = min(static_cast<int>(s.len) - 1, __ldg(a.row_limit + s.s0 + jl));
+    const int lim = limit_of(a, s, jl);
     float m_run = -INFINITY, l_run = 0.0f;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
@@ -494,7 +594,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     if (ok && mbar_wait(&bars->o_full, 0, abort)) {
       tc_fence_after();
       if (bars->v_poison <= lim) l_run = __uint_as_float(0x7FC00000u);
-      const float inv = l_run == 0.0f ? 0.0f : bfp16_scale(static_cast<uint32_t>(bars->e_max)) / l_run;
+      // (two factors: their product may leave the range of a float)
+      const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run, unit = bfp16_scale(static_cast<uint32_t>(bars->e_max)) * 0x1p-5f;
+      static_assert(kUpV == 5, "unit of O");
       uint16_t* orow = a.o + (s.s0 + jr) * a.ldo + (h * a.group.d + row - jr * a.group.d) * HD;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -505,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            w[i] = attn::pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            w[i] = attn::pack_bf16x2(__uint_as_float(o[2 * i]) * inv * unit, __uint_as_float(o[2 * i + 1]) * inv * unit);
           if (a.vec) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)

@@ -74,6 +74,41 @@ def test_hidden_values_far_above(env, form, masks, kv, new, H, hkv, page):
     hidden_values(env, form, 180, masks, kv, new, H, hkv, page)
 
 
+@pytest.mark.parametrize("kv,new,H,hkv,page", HIDDEN)
+@pytest.mark.parametrize("masks", ["causal", "row_limit"])
+@pytest.mark.parametrize("spread", [4, 24, 25, 29, 30, 31, 40, 100, 180])
+@pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
+def test_hidden_values(env, form, spread, masks, kv, new, H, hkv, page):
+    hidden_values(env, form, spread, masks, kv, new, H, hkv, page)
+
+
+@pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
+def test_hidden_values_beside_absent_and_poisoned_blocks(env, form):
+    """Values far apart, a page outside the pool among the low and one among the high ones, a block with a NaN behind; q and
+    the output with strides of their own."""
+    torch, ops, L, dev = env
+    c = Case(torch, ops, dev, [330, 40], [300, 40], 2, 16, seed=13)
+    value_exponents(c, torch, dev, lambda b, pos: 150 if pos >= 192 else 110)
+    table = c.table.copy()
+    table[0, 3], table[0, 13] = -1, c.pages
+    present = [np.ones(330, bool), np.ones(40, bool)]
+    present[0][48:64] = present[0][208:224] = False
+    c.pool.v_exp[0, int(table[0, 17])] = 255                           # positions 272 .. 287
+    q = O.bf16_round(c.rng.standard_normal((c.T, 4, 128)).astype(np.float32))
+    out = torch.full((c.T, 523), 7.0, dtype=torch.bfloat16, device=dev)
+    attend(ops, form, bf16(torch, q.transpose(1, 0, 2).copy(), dev).transpose(0, 1), c.pool, 0, torch.from_numpy(table).to(dev),
+           c.d_len, c.d_start, out=out[:, 1:513])
+    with pytest.raises(L.RedlineError, match="range check"):
+        ops.device_status()
+    assert (out[:, 0] == 7).all() and (out[:, 513:] == 7).all()
+    ref, tol = c.oracle(q, present=present)
+    sees = np.arange(c.T) + 30 >= 272
+    sees[300:] = False
+    got = out[:, 1:513].float().cpu().numpy().reshape(ref.shape)
+    assert np.isnan(got[sees]).all()
+    check_attention(torch.from_numpy(got[~sees]), ref[~sees], tol[~sees])
+
+
 @pytest.mark.parametrize("kv,new,H", [([3000], [1], 4), ([2000, 900], [40, 300], 2)])
 @pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
 def test_values_near_the_largest(env, form, kv, new, H):
