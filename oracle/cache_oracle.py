@@ -75,9 +75,11 @@ def attention(q, k, v, limit, present=None):
     the error that half-step fp16 weights and fp32 scores leave before the output's own rounding:
     2 * 2^-11 * sum w|v| (each weight and the sum of weights off by 2^-11), the scores' fp32 sums of 128 products (128
     half steps of 2^-24 of sum |q k|, doubled for the tensor core's truncation) carried through the exponential into
-    weights and sum, and weights below fp16's normal range: weights are kept times 2^4 and, in a block whose V exponent is
-    d <= 8 below the largest, times 2^-d, so they are off by 2^-25 2^(d - 4) there (the largest weight being >= 1) and
-    |v| <= 2^(E - d - 126) for the largest exponent E: together at most 2^-29 2^(E - 126) <= 2^-28 max |v| a key."""
+    weights and sum, and weights below fp16's normal range: the split kernel keeps weights times 2^4 and, in a block whose
+    V exponent is d <= 8 below the largest, times 2^-d, so they are off by 2^-25 2^(d - 4) there (the largest weight being
+    >= 1) and |v| <= 2^(E - d - 126) for the largest exponent E: together at most 2^-29 2^(E - 126) <= 2^-28 max |v| a key.
+    The prompt kernel keeps them times 2^7 (off by 2^-32 of the largest) and takes blocks whose values are below 2^-29 of the
+    largest as zeros, which is no more."""
     n, heads, _ = q.shape
     grp = heads // k.shape[1]
     o, bound = np.zeros(q.shape), np.zeros(q.shape)

@@ -15,7 +15,9 @@
 //    reaches a row. Both are written [key][64 dims] with the 128-byte swizzle: K-major for S, and for P V the
 //    same layout read as MN-major B. The codes wait in the converters' registers for the time of a block (with one item in
 //    flight their latency bound the kernel: 791 us for the case below, staged through shared memory 346).
-//  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding (half a step, 2^-11 of each weight).
+//  * P is fp16 (11 significant bits), V too; the row sum adds P before its rounding. P is kept times 2^kUpP (at most
+//    2^(kTau + kUpP) = 2^15), so a weight is off by half a step, 2^-11 of it, down to 2^-21 of the row's largest and by
+//    2^-32 of the largest below that: without it weights below 2^-25 were lost whole, 0.4 % of the row in a tail of 131072.
 //  * the tile's rows need not be consecutive in memory, so Q is copied by plain loads, all warps taking part.
 //
 // The chain of a tile bounds it, 4000 cycles per block of both tiles: softmax 2700 (it shares the issue slots and the shared
@@ -51,6 +53,7 @@ constexpr int kBytes = 1024 + kBar + 1024;
 static_assert(kBytes <= 232448, "shared memory");
 constexpr int kTmemCols = 512, kOCol = 256;
 constexpr float kTau = 8.0f;
+constexpr float kUpP = 7.0f;
 constexpr int kUpV = 5;               // V is kept times 2^kUpV: 1152 2^kUpV, the offset, has to be an fp16 number
 constexpr int kReach = 24 + kUpV;
 constexpr int kConv = 3;              // converter warps: 0, 2 and 3 (1 issues the MMAs)
@@ -186,7 +189,7 @@ __device__ __forceinline__ void softmax_block(uint32_t ta, uint32_t to, int key0
     m_run = mx;
   }
   const bool rescale = o_live && __any_sync(0xffffffffu, raise);
-  const float mz = m_run == -INFINITY ? 0.0f : m_run;             // a row that has seen no key: every score is -inf
+  const float mz = m_run == -INFINITY ? 0.0f : m_run - kUpP;      // a row that has seen no key: every score is -inf
   const float2 nm2 = make_float2(-mz, -mz);
   float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll

@@ -120,3 +120,27 @@ def test_values_near_the_largest(env, form, kv, new, H):
     got = attend(ops, form, bf16(torch, q, dev), *c.args())
     ops.device_status()
     check_attention(got, *c.oracle(q))
+
+
+@pytest.mark.parametrize("weight", [-22.3, -24.9, -25.0, -26.5])
+@pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
+def test_a_long_tail_of_small_weights(env, form, weight):
+    """One key holds nearly all of the softmax, 131071 others 2^weight of it each: their values count."""
+    torch, ops, L, dev = env
+    n = 131072
+    c = Case(torch, ops, dev, [n], [1], 1, 64, seed=7)
+    sink = c.table[0, 0]
+    for cache, codes, exps in ((c.k, c.pool.k, c.pool.k_exp), (c.v, c.pool.v, c.pool.v_exp)):
+        cache.exps[:] = 133                                          # values are codes - 128
+        cache.codes[:] = 128 if cache is c.k else 128 + 100
+        if cache is c.k:
+            cache.codes[sink, 0, 0, :64] = 129                       # the first key's score
+        else:
+            cache.codes[sink, 0, 0] = 128                            # and its value, zero
+        codes[0] = torch.from_numpy(cache.codes).to(dev)
+        exps[0] = torch.from_numpy(cache.exps).to(dev)
+    q = np.zeros((1, 2, 128), np.float32)
+    q[:, :, :64] = O.bf16_round(np.full(64, -weight * np.log(2) * np.sqrt(128) / 64, np.float32))
+    got = attend(ops, form, bf16(torch, q, dev), *c.args())
+    ops.device_status()
+    check_attention(got, *c.oracle(q))
