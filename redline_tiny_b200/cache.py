@@ -41,14 +41,15 @@ class PagedKV:
         self._seqs = {}                    # sequence -> its pages in order
         self._len = {}
         self._next = 0
-        self._version = 0                  # grows when pages move: a batch's tables are then out of date
+        self._version = 0                  # grows when any sequence's pages or length change
+        self._stamp = {}                   # sequence -> the version of its last change: what a batch's tables go by
 
     # -- books ------------------------------------------------------------------------------------------------------
     def new(self):
         """An empty sequence."""
         s = self._next
         self._next += 1
-        self._seqs[s], self._len[s] = [], 0
+        self._seqs[s], self._len[s], self._stamp[s] = [], 0, self._version
         return s
 
     def fork(self, seq):
@@ -64,7 +65,8 @@ class PagedKV:
         """Give up a sequence; pages that no other sequence holds are free again."""
         self.length(seq)
         self._release(self._seqs.pop(seq))
-        del self._len[seq]
+        del self._len[seq], self._stamp[seq]
+        self._version += 1
 
     def truncate(self, seq, length):
         """Forget the tokens from position `length` on."""
@@ -73,7 +75,14 @@ class PagedKV:
         pages, keep = self._seqs[seq], -(-length // self.page)
         self._release(pages[keep:])
         del pages[keep:]
-        self._len[seq] = length
+        if length != self._len[seq]:
+            self._len[seq] = length
+            self._changed([seq])
+
+    def _changed(self, seqs):
+        self._version += 1
+        for s in seqs:
+            self._stamp[s] = self._version
 
     def _release(self, pages):
         for p in pages:
@@ -127,6 +136,7 @@ class PagedKV:
                 self.refs[q] = 1
                 pages.append(q)
             self._len[s] = have + n
+        self._changed(s for s, n in zip(seqs, counts) if n)
         return copies
 
     def compact(self):
@@ -140,10 +150,10 @@ class PagedKV:
             ops.kv_copy_pages(self.pool, list(to.keys()), list(to.values()))
             for p, q in to.items():
                 self.refs[q], self.refs[p] = self.refs[p], 0
+            self._changed([s for s, pages in self._seqs.items() if any(p in to for p in pages)])
             for pages in self._seqs.values():
                 pages[:] = [to.get(p, p) for p in pages]
             self._free = list(range(n, len(self.refs)))
-            self._version += 1
         return len(to)
 
     def resize(self, pages):
@@ -164,7 +174,8 @@ class PagedKV:
 
 class Batch:
     """Sequences that take steps together. `args` = (table, kv_len, q_start): the device arrays that ops.kv_append and
-    ops.kv_attention take, at addresses that never change."""
+    ops.kv_attention take, at addresses that never change. They hold what the last `extend` left: once a sequence's pages
+    or length have changed otherwise (another batch's extend, truncate, free, compact), `args` raises until the next."""
 
     def __init__(self, kv, seqs, max_pages):
         self.kv, self.seqs = kv, list(seqs)
@@ -177,7 +188,8 @@ class Batch:
         self._meta = torch.full((B * self.width + 2 * B + 1,), -1, dtype=torch.int32, device=dev)
         self._meta[B * self.width:] = 0
         self._written = [[] for _ in self.seqs]      # what the device tables hold
-        self._lens, self._starts, self._version = [0] * B, [0] * (B + 1), kv._version
+        self._lens, self._starts = [0] * B, [0] * (B + 1)
+        self._version, self._stamps = kv._version, [kv._stamp[s] for s in self.seqs]
         self.table = self._meta[:B * self.width].view(B, self.width)
         self.kv_len = self._meta[B * self.width:B * self.width + B]
         self.q_start = self._meta[B * self.width + B:]
@@ -185,7 +197,10 @@ class Batch:
     @property
     def args(self):
         if self._version != self.kv._version:
-            raise RuntimeError("the cache's pages have moved since this batch's last extend")
+            for s, t in zip(self.seqs, self._stamps):
+                if self.kv._stamp.get(s) != t:
+                    raise RuntimeError(f"the pages or the length of sequence {s} have moved since this batch's last extend")
+            self._version = self.kv._version
         return self.table, self.kv_len, self.q_start
 
     @property
@@ -227,6 +242,6 @@ class Batch:
             if self._starts[b] != at:
                 self._starts[b] = new[B * W + B + b] = at
             at += counts[b] if b < B else 0
-        self._version = kv._version
+        self._version, self._stamps = kv._version, [kv._stamp[s] for s in self.seqs]
         if new:
             ops.kv_set(self._meta, new)
