@@ -107,8 +107,9 @@ class PagedKV:
         """A batch of different sequences; `max_pages` bounds the pages of each (default: the whole pool)."""
         return Batch(self, seqs, max_pages or len(self.refs))
 
-    def _extend(self, seqs, counts):
-        """Room for counts[i] more tokens of seqs[i]: (page, its private copy) pairs to copy."""
+    def _plan(self, seqs, counts):
+        """What room for counts[i] more tokens of seqs[i] takes, with nothing changed: per sequence (the page that its tail
+        moves to or None, new pages), and the (page, its private copy) pairs to copy first."""
         fresh, shared = 0, {}
         for s, n in zip(seqs, counts):
             if n < 0:
@@ -122,22 +123,31 @@ class PagedKV:
         copies_needed = sum(min(c, self.refs[p] - 1) for p, c in shared.items())
         if fresh + copies_needed > len(self._free):
             raise OutOfPages(f"{fresh + copies_needed} pages needed, {len(self._free)} free")
-        copies = []
+        take = iter(heapq.nsmallest(fresh + copies_needed, self._free))
+        holders, moves, copies = {}, [], []
         for s, n in zip(seqs, counts):
-            have, pages = self._len[s], self._seqs[s]
-            if n and have % self.page and self.refs[pages[-1]] > 1:
-                p, q = pages[-1], heapq.heappop(self._free)
-                self.refs[p] -= 1
-                self.refs[q] = 1
-                pages[-1] = q
-                copies.append((p, q))
-            for _ in range(-(-(have + n) // self.page) - len(pages)):
-                q = heapq.heappop(self._free)
-                self.refs[q] = 1
-                pages.append(q)
-            self._len[s] = have + n
-        self._changed(s for s, n in zip(seqs, counts) if n)
-        return copies
+            have, pages, tail = self._len[s], self._seqs[s], None
+            if n and have % self.page:
+                p = pages[-1]
+                left = holders.get(p, self.refs[p])
+                if left > 1:
+                    holders[p], tail = left - 1, next(take)
+                    copies.append((p, tail))
+            moves.append((tail, [next(take) for _ in range(-(-(have + n) // self.page) - len(pages))]))
+        return moves, copies
+
+    def _commit(self, seqs, counts, moves):
+        for s, n, (tail, more) in zip(seqs, counts, moves):
+            pages = self._seqs[s]
+            if tail is not None:
+                self.refs[pages[-1]] -= 1
+                pages[-1] = tail
+            pages += more
+            for p in more if tail is None else [tail, *more]:
+                self.refs[p] = 1
+                heapq.heappop(self._free)          # (the plan took the lowest)
+            self._len[s] += n
+        self._changed([s for s, n in zip(seqs, counts) if n])
 
     def compact(self):
         """Move the live pages to the front of the pool, so that its tail can be given back (resize). Returns the number
@@ -188,7 +198,7 @@ class Batch:
         self._meta = torch.full((B * self.width + 2 * B + 1,), -1, dtype=torch.int32, device=dev)
         self._meta[B * self.width:] = 0
         self._written = [[] for _ in self.seqs]      # what the device tables hold
-        self._lens, self._starts = [0] * B, [0] * (B + 1)
+        self._lens, self._starts, self._rows = [0] * B, [0] * (B + 1), 0
         self._version, self._stamps = kv._version, [kv._stamp[s] for s in self.seqs]
         self.table = self._meta[:B * self.width].view(B, self.width)
         self.kv_len = self._meta[B * self.width:B * self.width + B]
@@ -206,11 +216,12 @@ class Batch:
     @property
     def rows(self):
         """New tokens of the last extend."""
-        return self._starts[-1]
+        return self._rows
 
     def extend(self, counts):
         """Make room for counts[i] new tokens of each sequence and point the device arrays at them: pages are taken,
-        shared pages that will be written are copied. Raises OutOfPages, with nothing changed, where the pool is full."""
+        shared pages that will be written are copied. Raises OutOfPages where the pool is full; an extend that raises leaves
+        the cache's books as they were."""
         _not_captured("extend")
         counts = list(counts)
         kv, B = self.kv, len(self.seqs)
@@ -222,26 +233,52 @@ class Batch:
                 raise OutOfPages(f"sequence {s} needs {need} pages of a pool of {len(kv.refs)}")
             if need > self.width:
                 raise ValueError(f"sequence {s} would need more than the batch's {self.width} pages a sequence")
-        copies = kv._extend(self.seqs, counts)
+        moves, copies = kv._plan(self.seqs, counts)
+        # the device first, the books when all its calls have been taken
         if copies:
             ops.kv_copy_pages(kv.pool, [a for a, _ in copies], [b for _, b in copies])
-        self._write(counts)
-
-    def _write(self, counts):
-        kv, B, W, new = self.kv, len(self.seqs), self.width, {}
-        for b, s in enumerate(self.seqs):
-            pages, have = kv._seqs[s], self._written[b]
-            for i, p in enumerate(pages):
-                if i >= len(have) or have[i] != p:
-                    new[b * W + i] = p
-            self._written[b] = list(pages)
-            if self._lens[b] != kv.length(s):
-                self._lens[b] = new[B * W + b] = kv.length(s)
-        at = 0
-        for b in range(B + 1):
-            if self._starts[b] != at:
-                self._starts[b] = new[B * W + B + b] = at
-            at += counts[b] if b < B else 0
+        entries, current, lens, starts = self._entries(counts, moves)
+        if entries:
+            try:
+                ops.kv_set(self._meta, entries)
+            except Exception:
+                self._forget()
+                raise
+        kv._commit(self.seqs, counts, moves)
+        for b, (tail, more) in enumerate(moves):
+            row = self._written[b]
+            if not current[b]:
+                row[:] = kv._seqs[self.seqs[b]]
+            else:
+                if tail is not None:
+                    row[-1] = tail
+                if more:
+                    row += more
+        self._lens, self._starts, self._rows = lens, starts, starts[-1]
         self._version, self._stamps = kv._version, [kv._stamp[s] for s in self.seqs]
-        if new:
-            ops.kv_set(self._meta, new)
+
+    def _forget(self):
+        """What the device arrays hold is not known: `args` raises, and the next extend writes them whole."""
+        B = len(self.seqs)
+        self._written, self._lens, self._starts = [[] for _ in range(B)], [None] * B, [None] * (B + 1)
+        self._version, self._stamps = None, [None] * B
+
+    def _entries(self, counts, moves):
+        """The entries of the device arrays that the planned step changes, and the lengths and row ranges that follow."""
+        kv, W, at, new, current, lens, starts = self.kv, self.width, 0, {}, [], [], [0]
+        for s, n, (tail, more), have, stamp in zip(self.seqs, counts, moves, self._written, self._stamps):
+            pages = kv._seqs[s]
+            k = len(pages)
+            same = stamp == kv._stamp[s] and len(have) == k          # the row holds the sequence's pages
+            if not same:
+                new.update((at + i, p) for i, p in enumerate(pages) if i >= len(have) or have[i] != p)
+            if tail is not None:
+                new[at + k - 1] = tail
+            for i, p in enumerate(more, at + k):
+                new[i] = p
+            at += W
+            current.append(same)
+            lens.append(kv._len[s] + n)
+            starts.append(starts[-1] + n)
+        new.update((at + i, v) for i, (v, old) in enumerate(zip(lens + starts, self._lens + self._starts)) if v != old)
+        return new, current, lens, starts

@@ -79,3 +79,37 @@ def test_other_sequences_do_not_matter(fake):  # noqa: F811
     assert table[0, 0] == kv.pages(a)[0] and lens.tolist() == [PAGE]
     assert kv.compact() == 0
     batch.args
+
+
+@pytest.mark.parametrize("call", ["kv_copy_pages", "kv_set"])
+def test_a_step_whose_device_calls_fail(fake, monkeypatch, call):  # noqa: F811
+    """No page is taken and no tail moved; the same step then succeeds, with tables that are right from end to end."""
+    kv, a, batch = cached(PAGE + 3)
+    fork = kv.fork(a)
+    step = kv.batch([fork, a])
+    step.extend([0, 0])
+    state = lambda: (kv.refs[:], sorted(kv._free), {s: (kv.pages(s), kv.length(s)) for s in (a, fork)})  # noqa: E731
+    before = state()
+    real = getattr(ops, call)
+
+    def partly(*args):
+        if call == "kv_set":
+            real(args[0], dict(list(args[1].items())[:2]))       # some entries are written before the failure
+        raise RuntimeError("no device")
+    monkeypatch.setattr(ops, call, partly)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no device"):
+            step.extend([PAGE, 1])
+        assert state() == before
+    monkeypatch.setattr(ops, call, real)
+    batch.args                                                   # the books did not move
+    if call == "kv_set":
+        refused(step)
+    step.extend([PAGE, 1])
+    append(kv, step, list(range(200, 200 + PAGE + 1)))
+    assert read(kv, fork) == list(range(PAGE + 3)) + list(range(200, 200 + PAGE))
+    assert read(kv, a) == list(range(PAGE + 3)) + [200 + PAGE]
+    table, lens, starts = (t.tolist() for t in step.args)
+    for row, s in zip(table, (fork, a)):
+        assert row[:len(kv.pages(s))] == list(kv.pages(s))
+    assert lens == [kv.length(fork), kv.length(a)] and starts == [0, PAGE, PAGE + 1] and step.rows == PAGE + 1
