@@ -104,7 +104,7 @@ class PagedKV:
 
     # -- steps ------------------------------------------------------------------------------------------------------
     def batch(self, seqs, max_pages=None):
-        """A batch of different sequences; `max_pages` bounds the pages of each (default: the whole pool)."""
+        """A batch of up to 1024 different sequences; `max_pages` bounds the pages of each (default: the whole pool)."""
         return Batch(self, seqs, max_pages or len(self.refs))
 
     def _plan(self, seqs, counts):
@@ -191,6 +191,10 @@ class Batch:
         self.kv, self.seqs = kv, list(seqs)
         if len(set(self.seqs)) != len(self.seqs):
             raise ValueError("a sequence appears twice in a batch")
+        if len(self.seqs) > ops.KV_SEQUENCES:     # (the kernels' limit, before the books depend on it)
+            raise ValueError(f"{len(self.seqs)} sequences in a batch (at most {ops.KV_SEQUENCES})")
+        if max_pages < 1 or max_pages * kv.page > ops.KV_TOKENS:
+            raise ValueError(f"{max_pages} pages a sequence (1 to {ops.KV_TOKENS // kv.page})")
         for s in self.seqs:
             kv.length(s)
         B, self.width = len(self.seqs), int(max_pages)

@@ -340,6 +340,7 @@ def _check_int32(name, t, *shape):
 
 
 KV_BLOCK = 16   # tokens of one K/V head that share an exponent
+KV_SEQUENCES, KV_TOKENS = 1024, 1 << 30   # the most that a call takes, and that a sequence's page table spans
 
 
 class KVPool:

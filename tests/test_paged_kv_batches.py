@@ -113,3 +113,16 @@ def test_a_step_whose_device_calls_fail(fake, monkeypatch, call):  # noqa: F811
     for row, s in zip(table, (fork, a)):
         assert row[:len(kv.pages(s))] == list(kv.pages(s))
     assert lens == [kv.length(fork), kv.length(a)] and starts == [0, PAGE, PAGE + 1] and step.rows == PAGE + 1
+
+
+def test_batches_that_no_kernel_takes(fake):  # noqa: F811
+    """More sequences, or tables for more tokens, than a kernel takes: refused when the batch is made, before any extend."""
+    kv = cache.PagedKV(1, 4, 1, PAGE, "cpu")
+    seqs = [kv.new() for _ in range(1025)]
+    with pytest.raises(ValueError, match="1025 sequences"):
+        kv.batch(seqs)
+    assert len(kv.batch(seqs[1:], max_pages=1).seqs) == 1024
+    for pages in (-1, (1 << 26) + 1):
+        with pytest.raises(ValueError, match="pages a sequence"):
+            kv.batch(seqs[:1], max_pages=pages)
+    assert kv.batch(seqs[:1]).width == 4
