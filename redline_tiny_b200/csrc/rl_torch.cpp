@@ -12,6 +12,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstring>
+
 #include "../../include/redline_b200.h"
 
 namespace {
@@ -179,6 +181,23 @@ PyMethodDef kMethods[] = {RL_METHOD(kv_append), RL_METHOD(kv_read), RL_METHOD(kv
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_rl_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
+#define RL_STR_(x) #x
+#define RL_STR(x) RL_STR_(x)
+constexpr char kPython[] = RL_STR(PY_MAJOR_VERSION) "." RL_STR(PY_MINOR_VERSION) ".";
+
 }  // namespace
 
-PyMODINIT_FUNC PyInit__rl_torch() { return PyModule_Create(&kModule); }
+// Refuses to load beside another torch or Python than it was built for: tensors are reached through their headers.
+PyMODINIT_FUNC PyInit__rl_torch() {
+  PyObject* m = PyImport_ImportModule("torch.version");
+  PyObject* v = m ? PyObject_GetAttrString(m, "__version__") : nullptr;
+  PyObject* s = v ? PyObject_Str(v) : nullptr;
+  const char* have = s ? PyUnicode_AsUTF8(s) : nullptr;
+  const bool same = have && std::strcmp(have, RL_TORCH_VERSION) == 0 &&
+                    std::strncmp(Py_GetVersion(), kPython, sizeof(kPython) - 1) == 0;
+  if (have && !same)
+    PyErr_Format(PyExc_ImportError, "_rl_torch is built for torch %s and Python %s, not for torch %s and Python %s",
+                 RL_TORCH_VERSION, kPython, have, Py_GetVersion());
+  Py_XDECREF(s), Py_XDECREF(v), Py_XDECREF(m);
+  return same ? PyModule_Create(&kModule) : nullptr;
+}
