@@ -189,6 +189,10 @@ class CachedLM:
         if batch.kv is not self.kv or T != batch.rows:
             raise ValueError(f"{T} rows for a batch with {batch.rows} new tokens" if batch.kv is self.kv else
                              "the batch belongs to another cache")
+        if x.shape != (T, cfg.hidden) or x.dtype is not torch.bfloat16:
+            raise ValueError(f"x must be bf16 (rows, {cfg.hidden}), not {x.dtype} {tuple(x.shape)}")
+        if cos.shape != (T, HEAD_DIM // 2) or sin.shape != cos.shape:
+            raise ValueError(f"cos and sin must be ({T}, {HEAD_DIM // 2}), not {tuple(cos.shape)} and {tuple(sin.shape)}")
         if T == 0:
             return x
         rope = torch.stack([cos.float(), sin.float()], -1).reshape(T, 128).contiguous()
