@@ -169,11 +169,17 @@ struct WideBlock {
 
 // One warp per (group of `rows` rows, head, K or V). A row leads when it is the first of its block among the new
 // tokens; the warp writes the blocks of its leading rows: the block's new values are read once into registers, their
-// largest exponent field is joined with the exponent of the older tokens of the block, and the codes are stored.
+// largest exponent field is joined with the exponent of the older tokens of the block, and the codes are stored. The last
+// CTA reports impossible sequences, whichever rows they claim.
 template <typename Block>
 __global__ void __launch_bounds__(128) append_kernel(const Source sk, const Source sv, const Pool p, const Batch bt,
                                                      int rows, int64_t groups) {
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int b = threadIdx.x; b < bt.B; b += blockDim.x)
+      if (!load_seq(bt, b, p.page).ok) report(kErrBadArgument);
+    return;
+  }
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   if (w >= groups * p.hkv * 2) return;
   const int is_v = static_cast<int>(w & 1);
@@ -194,7 +200,6 @@ __global__ void __launch_bounds__(128) append_kernel(const Source sk, const Sour
     while (b + 1 < bt.B && r >= s.s0 + s.n) s = load_seq(bt, ++b, p.page);
     if (r < s.s0 || r >= s.s0 + s.n) { ++r; continue; }   // a row of no sequence
     if (!s.ok) {
-      if (lane == 0) report(kErrBadArgument);
       r = s.s0 + s.n;
       continue;
     }
@@ -385,7 +390,7 @@ int rl_kv_append(const void* k, int64_t k_st, int64_t k_sh, int64_t k_sd, const 
   const int64_t ctas = (groups * kv_heads * 2 + 3) / 4;
   const kv::Source sk{k, k_st, k_sh, k_sd}, sv{v, v_st, v_sh, v_sd};
   auto wide = [](const kv::Source& s) { return s.sd == 1 && aligned(s.x, 16) && s.st % 8 == 0 && s.sh % 8 == 0; };
-  const unsigned grid = static_cast<unsigned>(ctas);
+  const unsigned grid = static_cast<unsigned>(ctas) + 1;
   if (dtype == RL_BF16 && wide(sk) && wide(sv))
     kv::append_kernel<kv::WideBlock><<<grid, 128, 0, stream>>>(sk, sv, p, bt, rows, groups);
   else if (dtype == RL_BF16)
