@@ -378,6 +378,7 @@ int rl_kv_append(const void* k, int64_t k_st, int64_t k_sh, int64_t k_sd, const 
   int st;
   if ((st = kv::check_pool("rl_kv_append", p)) != RL_OK || (st = kv::check_batch("rl_kv_append", bt)) != RL_OK) return st;
   RL_REQUIRE(dtype == RL_F32 || dtype == RL_BF16, RL_ERR_ARGUMENT, "rl_kv_append: unknown dtype %d", dtype);
+  RL_REQUIRE(T * kv_heads < (1ll << 35), RL_ERR_ARGUMENT, "rl_kv_append: %lld rows of %d heads", (long long)T, kv_heads);
   if (T == 0 || B == 0) return RL_OK;
   RL_REQUIRE(k && v && q_start, RL_ERR_ARGUMENT, "rl_kv_append: NULL pointer");
   const uintptr_t es = dtype == RL_F32 ? 4 : 2;
