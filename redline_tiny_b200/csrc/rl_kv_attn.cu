@@ -199,13 +199,7 @@ struct Acc {
   float o[NT][8][4];     // O^T: dims 16g + 2i (+1 for [2], [3]), rows 2c, 2c + 1 of n-tile nt
   float m[NT][2], l[NT][2];
   int er;                // the largest V exponent of the warp's blocks so far
-  uint32_t unit[(NT + 1) / 2];   // O of a row is in units of 2^(unit - 133), a byte a row: er of the last block that it sees
-
-  __device__ __forceinline__ int unit_of(int nt, int c) const { return unit[nt >> 1] >> (16 * (nt & 1) + 8 * c) & 255u; }
-  __device__ __forceinline__ void set_unit(int nt, int c, int e) {
-    const int sh = 16 * (nt & 1) + 8 * c;
-    unit[nt >> 1] = (unit[nt >> 1] & ~(255u << sh)) | static_cast<uint32_t>(e) << sh;
-  }
+  int unit[NT][2];       // O of a row is in units of 2^(unit - 133): er of the last block that the row sees
 };
 
 // P^T of a block times 2^shift, in the B layout; the row sums add the weights, before their rounding, times `unit`.
@@ -294,7 +288,7 @@ __device__ __forceinline__ void block_step(const uint4 (&kr)[4], const uint4 (&v
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          if (pos0 <= lim[nt][c]) acc.set_unit(nt, c, ev);
+          acc.unit[nt][c] = pos0 <= lim[nt][c] ? ev : acc.unit[nt][c];
     }
     d = acc.er - ev;
 #pragma unroll
@@ -527,9 +521,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
           page_next = page_of(k + 32 + lane);
         }
         const int found = __shfl_sync(0xffffffffu, idx, k & 31);
-        const int64_t blk = max(found, 0);                           // an absent block reads as block 0, fully masked
+        // an absent block reads as block 0, fully masked, with an exponent (255) that moves no unit
+        const int64_t blk = max(found, 0);
         at_pos[j] = found < 0 ? 0x7FFFFF00 : static_cast<int>(pos0) + k * (kWarps * BT);
-        ke[j] = a.pool.ke[blk], ve[j] = a.pool.ve[blk];
+        ke[j] = a.pool.ke[blk], ve[j] = 255u;
+        if (found >= 0) ve[j] = a.pool.ve[blk];
         const uint8_t* kp = a.pool.k + blk * (BT * HD) + lane * 16;
         const uint8_t* vp = a.pool.v + blk * (BT * HD) + lane * 16;
         const uint32_t d = ring + j * (2 * BT * HD) + wr * HD;
@@ -564,7 +560,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
     Acc<NT> acc;
     acc.er = 0;
 #pragma unroll
-    for (int i = 0; i < (NT + 1) / 2; ++i) acc.unit[i] = 0;
+    for (int nt = 0; nt < NT; ++nt) acc.unit[nt][0] = acc.unit[nt][1] = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       acc.m[nt][0] = acc.m[nt][1] = kNone;
@@ -603,10 +599,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtas) attend_kern
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = nt * 8 + 2 * c + k;
-        const int unit = acc.unit_of(nt, k), over = max(unit - kMostUnit, 0);
+        const int unit = acc.unit[nt][k], over = max(unit - kMostUnit, 0);
         const float ou = bfp16_scale(static_cast<uint32_t>(unit - over));
-        l *= __uint_as_float(static_cast<uint32_t>(127 - over) << 23);
-        if (g == 0) sm[warp * R + row] = acc.m[nt][k] + static_cast<float>(over), sl[warp * R + row] = l;
+        float m = acc.m[nt][k];
+        if (over) l *= __uint_as_float(static_cast<uint32_t>(127 - over) << 23), m += static_cast<float>(over);
+        if (g == 0) sm[warp * R + row] = m, sl[warp * R + row] = l;
         float* d = so + (warp * R + row) * HD + 16 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i)

@@ -294,7 +294,7 @@ __device__ __noinline__ void far_tile(const Args& a, const int (&task)[6]) {
       for (int d = 4; d <= 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
       const uint32_t r = r0 + 2 * c + k, j = r / a.group;
       if (r >= end) continue;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = bfp16_scale(static_cast<uint32_t>(acc.unit_of(0, k)));
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = bfp16_scale(static_cast<uint32_t>(acc.unit[0][k]));
       uint16_t* o = a.o + (s.s0 + j) * a.ldo + (h * a.group.d + r - j * a.group.d) * HD + 16 * g;
 #pragma unroll
       for (int i = 0; i < 8; ++i)

@@ -144,3 +144,32 @@ def test_a_long_tail_of_small_weights(env, form, weight):
     got = attend(ops, form, bf16(torch, q, dev), *c.args())
     ops.device_status()
     check_attention(got, *c.oracle(q))
+
+
+# (the second and third have work for several blocks a warp, whose scales then meet)
+@pytest.mark.parametrize("kv,new,H", [([300, 90], [12, 3], 2), ([2000], [700], 4), ([2600] * 30, [1] * 30, 2)])
+@pytest.mark.parametrize("form", ["split", "prompt", "cluster"])
+def test_absent_pages_bring_no_scale_with_them(env, form, kv, new, H):
+    """A page outside the pool among a sequence's: what the kernels read in its place, large values or a NaN, counts for nothing."""
+    torch, ops, L, dev = env
+    for there in (140, 255):
+        c = Case(torch, ops, dev, kv, new, 1, 16, seed=19)
+        free = int(c.free[0])
+        order = [free] + [p for p in range(c.pages) if p != free]            # page 0 belongs to no sequence
+        for t in (c.pool.k, c.pool.v, c.pool.k_exp, c.pool.v_exp):
+            t[:] = t[:, order].clone()
+        for cache in (c.k, c.v):
+            cache.codes, cache.exps = cache.codes[order], cache.exps[order]
+        back = np.argsort(order)
+        c.table = np.where(c.table >= 0, back[c.table], -1).astype(np.int32)
+        c.pool.k_exp[0, 0], c.pool.v_exp[0, 0] = 255 if there == 255 else 127, there
+        table, present = c.table.copy(), [np.ones(a, bool) for a in kv]
+        for b, a in enumerate(kv):
+            for p in range(1, a // 16, 3):
+                table[b, p] = -1 if p % 2 else c.pages + 7
+                present[b][16 * p:16 * p + 16] = False
+        q = O.bf16_round((c.rng.standard_normal((c.T, H, 128)) * 0.1).astype(np.float32))
+        got = attend(ops, form, bf16(torch, q, dev), c.pool, 0, torch.from_numpy(table).to(dev), c.d_len, c.d_start)
+        with pytest.raises(L.RedlineError, match="range check"):
+            ops.device_status()
+        check_attention(got, *c.oracle(q, present=present))
