@@ -396,8 +396,9 @@ int rl_set_attention_variant(int variant);
  * A batch of B <= 1024 sequences lies in device memory: table (B rows of table_ld int32: the pages of the sequence in
  * order), kv_len[B] (tokens in the cache, the new ones included), q_start[B + 1] (the new tokens of sequence b are rows
  * q_start[b] .. q_start[b + 1] - 1; row j of n sits at position kv_len - n + j). The kernels check what they read: a
- * sequence whose numbers are impossible is left out, a page outside the pool is skipped (its keys count as absent), and
- * both are reported through rl_device_status. Rows of no sequence are neither read nor written.
+ * sequence whose numbers are impossible is left out (with row ranges that fall, its neighbours' rows may be too), a page
+ * outside the pool is skipped (its keys count as absent), and both are reported through rl_device_status. Rows of no sequence
+ * are neither read nor written.
  */
 
 /*
@@ -434,9 +435,12 @@ int rl_kv_set(int32_t* dst, int64_t size, const int32_t* at, const int32_t* valu
  * q: bf16, element (row, head, dim) at row * q_st + head * q_sh + dim, strides multiples of 8, 16-byte aligned.
  * Row j of n of a sequence sees the keys at positions <= kv_len - n + j, or, with row_limit (int32 [T]), those <=
  * min(row_limit[row], kv_len - 1). A row that sees no key gives zeros. o: bf16 (T, ldo), head h at columns 128h ..,
- * O / l rounded once (not to bfp16 blocks). Keys are weighted with P rounded to fp16; sums are fp32. Results do not
- * depend on timing. workspace: rl_kv_attention_workspace bytes, 16-byte aligned, needs no initialisation and holds
- * nothing between calls; calls that may run at the same time need workspaces of their own.
+ * O / l rounded once (not to bfp16 blocks). Keys are weighted with P rounded to fp16; sums are fp32. What a row's limit hides
+ * does not reach it; beside the roundings, a key may be off by 2^-28 of the largest value that the row sees. Results do not
+ * depend on timing. Rows of no sequence are left as they were. workspace: rl_kv_attention_workspace bytes, 16-byte aligned,
+ * needs no initialisation and holds nothing between calls; calls that may run at the same time need workspaces of their own.
+ * The kernel is chosen by the call's sizes alone: the fast form for short contexts needs table_ld * page <= 6144, and long
+ * chunks and single rows are better given to calls of their own than mixed in one.
  */
 size_t rl_kv_attention_workspace(int64_t T, int B, int heads, int kv_heads);
 /* Kernel choice, for tests and measurements: 0 = by shape, 1 = the split kernel, 2 = the prompt kernel (positive scales

@@ -104,7 +104,8 @@ class PagedKV:
 
     # -- steps ------------------------------------------------------------------------------------------------------
     def batch(self, seqs, max_pages=None):
-        """A batch of up to 1024 different sequences; `max_pages` bounds the pages of each (default: the whole pool)."""
+        """A batch of up to 1024 different sequences; `max_pages` bounds the pages of each (default: the whole pool). Attention
+        over short contexts is faster where that bound is at most 6144 tokens (777 keys: 5.6 against 7.0 us)."""
         return Batch(self, seqs, max_pages or len(self.refs))
 
     def _plan(self, seqs, counts):
@@ -151,7 +152,7 @@ class PagedKV:
 
     def compact(self):
         """Move the live pages to the front of the pool, so that its tail can be given back (resize). Returns the number
-        of pages moved. A batch follows at its next `extend` (of no tokens, if need be), not before."""
+        of pages moved. A batch whose pages moved follows at its next `extend` (of no tokens, if need be), not before."""
         _not_captured("compact")
         live = [p for p, r in enumerate(self.refs) if r]
         n = len(live)
@@ -167,7 +168,8 @@ class PagedKV:
         return len(to)
 
     def resize(self, pages):
-        """A pool of `pages` pages (compacted first when that drops any). Captured graphs hold the old one."""
+        """A pool of `pages` pages (compacted first when that drops any). The old pool's memory is given up: steps captured
+        before must not be replayed."""
         _not_captured("resize")
         if pages < len(self.refs):
             if pages < sum(1 for r in self.refs if r):
@@ -185,7 +187,8 @@ class PagedKV:
 class Batch:
     """Sequences that take steps together. `args` = (table, kv_len, q_start): the device arrays that ops.kv_append and
     ops.kv_attention take, at addresses that never change. They hold what the last `extend` left: once a sequence's pages
-    or length have changed otherwise (another batch's extend, truncate, free, compact), `args` raises until the next."""
+    or length have changed otherwise (another batch's extend, truncate, free, compact), `args` raises until the next. A
+    captured step reads the arrays as they are when it is replayed: extend comes before each replay."""
 
     def __init__(self, kv, seqs, max_pages):
         self.kv, self.seqs = kv, list(seqs)

@@ -22,7 +22,7 @@
 // Bound by the cache's bytes for one token a sequence: 269 MB (one sequence of 131071 tokens, 8 heads) in 54 us, of which
 // the loop over the keys takes 35 - 46 us a CTA (7.6 - 5.8 TB/s), its start 4 and the joins 5; 564 MB (64 sequences of up
 // to 8192) in 100 us = 5.7 TB/s. Steps, for the two: plain loads 114 / 166 us; copies through a per-warp ring 67 / 114; V
-// scales in P and no 64-bit divisions 55 / 102. A step of 777 keys takes 5.5 us in one launch of clusters (7.0 in two
+// scales in P and no 64-bit divisions 55 / 102. A step of 777 keys takes 5.6 us in one launch of clusters (7.0 in two
 // launches): the launch, three dependent loads, a block or two a warp, the joins.
 #include "rl_common.cuh"
 #include "rl_host.h"

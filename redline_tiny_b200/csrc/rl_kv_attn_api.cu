@@ -14,6 +14,8 @@ inline int& path() {   // 0 = by the rules below, 1 = split kernel, 2 = prompt k
 // The prompt kernel computes 256 rows x 128 keys in the time in which the split kernel, which runs on every SM whatever
 // the shape, gets through about a quarter of them: it pays where its tiles are more than a quarter full of rows and
 // the SMs more than a quarter full of tiles. (It scales row maxima, so it takes positive scales.)
+// It goes by the call's averages: 63 sequences of one row and one of 1021 take the prompt kernel for all, 279 us, where the
+// two kinds alone take 54 and 98; 63 without rows beside the same one fall to the split kernel, 424 us.
 inline bool by_prompt(int64_t T, int B, int heads, int kv_heads, float scale_log2) {
   if (!(scale_log2 > 0.0f) || path() == 1 || path() == 3) return false;
   if (path() == 2) return true;
@@ -24,9 +26,9 @@ inline bool by_prompt(int64_t T, int B, int heads, int kv_heads, float scale_log
   return full * (busy < 1.0 ? busy : 1.0) > 0.25;
 }
 
-// The one-launch form splits every task in eight, whatever its length: it wins while the page table bounds the keys and the
-// tasks' CTAs fit the GPU at once. Device times, spread over the grid / in clusters (32 heads over 8, one row a sequence):
-// 1 x 1024 keys 7.4 / 5.8 us, 1 x 4096 12.2 / 9.8, 1 x 8192 14.6 / 14.9, 2 x 8192 15.4 / 16.0, 8 x 4096 16.0 / 12.7,
+// The one-launch form splits every task in eight, whatever its length: it wins while the page table's width bounds the keys
+// (the lengths are in device memory) and the tasks' CTAs fit the GPU at once. Device times, spread over the grid / in clusters
+// (32 heads over 8, one row a sequence): 1 x 1024 keys 7.4 / 5.8 us, 1 x 4096 12.2 / 9.8, 1 x 8192 14.6 / 14.9, 2 x 8192 15.4 / 16.0, 8 x 4096 16.0 / 12.7,
 // 8 x 8192 20.7 / 19.0, 16 x 8192 34.5 / 35.4, 64 x 1024 33 / 53; 16 x up to 5 rows, 4097 keys, 8 over 2: 19.0 / 13.9.
 constexpr int64_t kShort = 6144;
 inline bool by_cluster(int nt, int64_t T, int B, int group, int hkv, int64_t most_keys) {

@@ -24,9 +24,10 @@
 // memory with the converters), the rest of P V and the next S 1300, about twice their arithmetic, since their operands and
 // the converters' stores share the shared memory too (the dense kernel takes 3300). A task adds 5.5 us until its first S and
 // about 2 behind its last block.
-// Three prompt chunks of 1021, 650 and 279 tokens over 8191, 5214 and 2245 (32 heads over 8): 233 us, 816 TFLOP/s; a fifth
+// Three prompt chunks of 1021, 650 and 279 tokens over 8191, 5214 and 2245 (32 heads over 8): 235 us, 809 TFLOP/s; a fifth
 // of it is the tail of 256 tasks of three lengths on 148 SMs. Steps: Q and the exponents by the converters alone, 272; by
-// all warps, loads ahead of stores, 242; the wait for K taken off the chain, 233. Rejected: reading S twice to free
+// all warps, loads ahead of stores, 242; the wait for K taken off the chain, 233; values and weights right over their whole
+// range, 235. A tile that goes by far_tile takes about 1.2 ms for 8191 keys. Rejected: reading S twice to free
 // registers (361 - 424 against 267), scales read from shared memory where they are used (280), part of the exponentials by a
 // polynomial (289 - 311 against 279), four converter warps (487), P handed over as 96 + 32 keys (248 against 233) or in
 // quarters (236), one thread for the issuer's waits (240), the first codes loaded ahead of the start's barrier (266).

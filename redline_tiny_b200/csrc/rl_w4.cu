@@ -1,8 +1,9 @@
-// Products of a few rows with 4-bit weights: C[m][n] = sum_k x[m][k] (u[n][k] - 8) s[n][k / G] (+ bias), m < 64.
+// Products of a few rows with 4-bit weights: C[m][n] = sum_k x[m][k] (u[n][k] - 8) s[n][k / G] (+ bias), m <= 64.
 //
-// Bound by the weight bytes (K N / 2) on paper at one row; what the kernels reach is set by the half-rate ALU pipe and the
-// latency of short streams: 50 MB of codes (4096 x 24576, one row) take 13.9 us = 3.8 TB/s with the ALU pipe at 44 % and
-// issue at 50 %, 12.6 MB (4096 x 6144) 4.6 - 5 us, of which a launch and one load are 4. The weights are the A operand of
+// Bound by the weight bytes (K N / 2) on paper at one row; the kernels stay above that floor with no unit saturated (ALU pipe
+// 44 %, issue 50 %): streams are short, and every CTA pays a start and a join for 16 columns. One row, weights from HBM / left
+// in the L2 by the call before: 50 MB of codes (4096 x 24576) 14.5 / 13.5 - 14.3 us = 3.7 TB/s, 12.6 MB (4096 x 6144)
+// 5.3 / 4.7 - 5.0 us, of which a launch and one load are 4. The weights are the A operand of
 // mma.m16n8k16 (16 columns of B on the M side, up to 8 rows of x per n-tile), turned from 4 bits to bf16 in registers,
 // exactly (nibbles_lo). A group's products are summed by the tensor core in fp32 and scaled once as they are added to the
 // fp32 result, so the only rounding is the output's (and fp32's). Rejected for one row: two column tiles a warp (17.4 us),
@@ -263,9 +264,12 @@ __global__ void __launch_bounds__(32 * kFew, 4) few_kernel(const Args a) {
 // 9 to 64 rows: one CTA per 128 columns and share of K, a warp per CT x 16 columns; the x of a share is brought into
 // shared memory once (with one warp per 16 columns reading x itself, x is M / 8 times the weights' bytes of L2 traffic)
 // and each fragment serves CT tiles of codes. The CTAs of a cluster hold the shares of K of the same columns and are
-// joined through distributed shared memory in rank order. 23 rows, 12288 x 4096: 14.3 us. mma.sync issues one m16n8k16 in
-// two cycles an SM (1024 products a cycle): 24 of them a tile and 192 tiles on the fullest SMs are 5 us, start, joins and
-// clusters that leave SMs empty the rest; 64 rows reach 200 - 226 TFLOP/s. Rejected: K split over warps as well (17 - 19 us).
+// joined through distributed shared memory in rank order. 23 rows, 12288 x 4096: 14.3 - 14.8 us, weights cold or not.
+// mma.sync issues one m16n8k16 in two cycles an SM (1024 products a cycle): 24 of them a tile and 192 tiles on the fullest SMs
+// are 5 us, start, joins and clusters that leave SMs empty the rest. 16 / 32 / 48 / 64 rows (groups of 64, weights cold):
+// 4096 x 24576 20.7 / 35.7 / 53.1 / 66.8 us, 12288 x 4096 13.4 / 16.5 / 23.9 / 28.8, 4096 x 6144 8.8 / 13.9 / 17.8 / 22.3. The
+// packed bfp16 GEMM takes 65, 28 and 22 us there at any of these row counts: at 64 rows the two meet. Rejected: K split over
+// warps as well (17 - 19 us).
 template <int NT>
 struct Many {
   static constexpr int CT = NT <= 3 ? 2 : 1;
@@ -327,7 +331,8 @@ __global__ void __launch_bounds__(Many<NT>::kThreads, Many<NT>::kCtas) many_kern
     for (int nt = 0; nt < NT; ++nt) acc[ct][nt][0] = acc[ct][nt][1] = acc[ct][nt][2] = acc[ct][nt][3] = 0.0f;
   const uint8_t* xa = smem + g * (TK * 2);
   const uint32_t xc = (c ^ ((g & 1) * 4)) << 4;
-  for (int p0 = t_begin; p0 < t_end; p0 += C::kPanel) {           // (one panel, unless K is very long)
+  // (few k tiles a share are one panel; 64 rows of 4096 x 24576 take three)
+  for (int p0 = t_begin; p0 < t_end; p0 += C::kPanel) {
     const int p1 = min(p0 + C::kPanel, t_end);
     if (p0 > t_begin) __syncthreads();                            // every warp is done with the panel before
     for (int t = p0; t < p1; ++t) {

@@ -455,8 +455,9 @@ def kv_attention(q, pool, layer, table, kv_len, q_start, row_limit=None, scale_l
     """Attention of new tokens q (T, heads, 128) bf16 (any row and head strides that are multiples of 8) over a layer of
     the cache, which holds their own keys already (kv_append). Row j of sequence b's n new rows sees positions
     <= kv_len[b] - n + j, or <= min(row_limit[row], kv_len[b] - 1) with row_limit int32 (T); a row that sees no key gives
-    zeros, a row of no sequence is left as it was. Returns bf16 (T, heads * 128); `out` must not overlap q. scale_log2
-    defaults to log2(e)/sqrt(128)."""
+    zeros; a row of no sequence is left as it was in `out`, and without `out` holds whatever its memory held. Returns bf16
+    (T, heads * 128); `out` must not overlap q. Contexts of up to 6144 tokens are fastest with a table no wider than that (the
+    kernel is chosen by shapes alone). scale_log2 defaults to log2(e)/sqrt(128)."""
     scale = _SCALE_LOG2 if scale_log2 is None else float(scale_log2)
     if _fast is not None and 0 <= layer < len(pool._fast):
         o = _fast.kv_attention(q, pool._fast[layer], table, kv_len, q_start, row_limit, scale, out)

